@@ -263,6 +263,57 @@ lc_status lc_gelu_backward(lc_context* ctx, void* stream, const lc_view* pre, co
 lc_status lc_relu(lc_context* ctx, void* stream, const lc_view* x, const lc_view* y);
 lc_status lc_relu_backward(lc_context* ctx, void* stream, const lc_view* pre, const lc_view* dy, const lc_view* dx);
 
+/* ---- scores and losses over a vocabulary (no reference counterpart) --------------------------- */
+/* `logits` is [..., V] of f32, f16 or bf16 with any strides: the last axis is the vocabulary (1 to
+ * 2^31 - 1 places), the leading axes are the rows.  The softmax is that of scale * logits, scale
+ * positive and finite (the inverse of a temperature); sums and statistics are f32 or wider.  Every
+ * other operand has the logits' leading shape, with one axis more where one is named.  Indices are
+ * i32 or u32; one outside [0, V), -1 among them, stands for no token.  Errors are the op API's
+ * (LC_ERR_INVALID_ARGUMENT, LC_ERR_OVERLAP); no output may overlap an input or another output, but
+ * dlogits may be the logits themselves (same buffer, offset, shape and strides).  The calls
+ * allocate nothing and may be captured into a graph.
+ * A logit of minus infinity is a masked place: its probability is 0.  In a row that is masked
+ * throughout every log probability is minus infinity, the entropy is 0 and the gradient is 0.  A
+ * NaN or plus infinity makes its row's results NaN. */
+
+/* Log probabilities of one token a row, the row's entropy and its best alternatives.  Every output
+ * may be NULL, not all of them:
+ *   logprob [...] f32        log p of targets[...]; 0 where there is no token (with targets only)
+ *   entropy [...] f32        -sum p log p
+ *   stats [..., 2] f32       the largest logit (not scaled) and log(sum e^(scale (x - largest))),
+ *                            for the gradient
+ *   top_logprobs [..., K] f32, top_ids [..., K]   the K largest logits' log probabilities and
+ *                            places, best first; equal logits by the lower place, a NaN above every
+ *                            number.  1 <= K <= 128, K <= V */
+lc_status lc_encode_token_logprobs(lc_context* ctx, void* stream, const lc_view* logits,
+                                   const lc_view* targets, float scale, const lc_view* logprob,
+                                   const lc_view* entropy, const lc_view* stats,
+                                   const lc_view* top_logprobs, const lc_view* top_ids);
+/* Its gradient: dlogits (the logits' type) = d_logprob * d(logprob)/d(logits) + d_entropy *
+ * d(entropy)/d(logits), from the `stats` (and `entropy`, where d_entropy is given) of the call
+ * above.  d_logprob (with targets) or d_entropy may be NULL, not both.  A row without a token has
+ * no gradient of its log probability. */
+lc_status lc_encode_token_logprobs_backward(lc_context* ctx, void* stream, const lc_view* logits,
+                                            const lc_view* targets, float scale, const lc_view* stats,
+                                            const lc_view* entropy, const lc_view* d_logprob,
+                                            const lc_view* d_entropy, const lc_view* dlogits);
+/* Distillation from a teacher's best alternatives: ids [..., K] and teacher [..., K] (f32, f16 or
+ * bf16), K at most 256.  An id that stands for no token is padding, and of an id that a row names
+ * twice the first entry stands.  With q = softmax(scale * logits), over the entries that stand:
+ *   tail 0: P = softmax(scale * teacher); loss [...] = sum P (log P - log q_id)
+ *   tail 1: teacher holds log probabilities, P = e^teacher; what they leave, r = max(0, 1 - sum P),
+ *           is one bucket against the student's Q outside the list:
+ *           loss = sum P (log P - log q_id) + r (log r - log Q), the bucket left out where Q = 0
+ * A row without entries has loss 0 (tail 0: and no gradient). */
+lc_status lc_encode_distill_loss(lc_context* ctx, void* stream, const lc_view* logits,
+                                 const lc_view* ids, const lc_view* teacher, float scale, int32_t tail,
+                                 const lc_view* loss);
+/* Its gradient in the same pass over the logits: dlogits (the logits' type) = d_loss * d(loss)/
+ * d(logits), d_loss [...] f32 (NULL: 1).  `loss` may be NULL. */
+lc_status lc_encode_distill_grad(lc_context* ctx, void* stream, const lc_view* logits,
+                                 const lc_view* ids, const lc_view* teacher, float scale, int32_t tail,
+                                 const lc_view* d_loss, const lc_view* loss, const lc_view* dlogits);
+
 /* ---- schedule, placement and wire (host-only) ---------------------------------------------- */
 
 /* `local_order` (crates/schedule/src/lib.rs:15-35): ops[i] = +(m+1) for Forward(m),

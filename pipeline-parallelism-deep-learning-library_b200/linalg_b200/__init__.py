@@ -139,6 +139,10 @@ def _sig(L):
         "lc_gelu_backward": (s, [_vp, _vp, _V, _V, _V]),
         "lc_relu": (s, [_vp, _vp, _V, _V]),
         "lc_relu_backward": (s, [_vp, _vp, _V, _V, _V]),
+        "lc_encode_token_logprobs": (s, [_vp, _vp, _V, _V, f, _V, _V, _V, _V, _V]),
+        "lc_encode_token_logprobs_backward": (s, [_vp, _vp, _V, _V, f, _V, _V, _V, _V, _V]),
+        "lc_encode_distill_loss": (s, [_vp, _vp, _V, _V, _V, f, C.c_int32, _V]),
+        "lc_encode_distill_grad": (s, [_vp, _vp, _V, _V, _V, f, C.c_int32, _V, _V, _V]),
         "lc_local_order": (s, [C.c_uint64, C.c_uint64, C.c_uint64, C.POINTER(C.c_int64), C.c_uint64,
                                C.POINTER(C.c_uint64)]),
         "lc_contiguous_placement": (s, [C.c_uint64, C.c_uint64, C.POINTER(C.c_uint64)]),
@@ -509,6 +513,63 @@ def gelu_backward(ctx, pre, dy, dx, stream=None):
 
 def relu_backward(ctx, pre, dy, dx, stream=None):
     check(load().lc_relu_backward(ctx.h, _stream(stream), as_view(pre).ref(), as_view(dy).ref(), as_view(dx).ref()))
+
+
+# ---------------------------------------------------------------------------------------------
+# scores and losses over a vocabulary (no reference counterpart)
+# ---------------------------------------------------------------------------------------------
+
+def _maybe(x):
+    """A view by reference, or NULL for an operand that is not there."""
+    return None if x is None else as_view(x).ref()
+
+
+def encode_token_logprobs(ctx: Context, stream, logits, targets, scale=1.0, logprob=None, entropy=None, stats=None,
+                          top_logprobs=None, top_ids=None):
+    """Log probabilities of ``targets`` under softmax(scale * logits) over the last axis, with the rows' entropy,
+    the ``stats`` that the gradient needs and the best alternatives; every output is optional, not all of them.
+    A target outside [0, V), such as -1, stands for no token."""
+    check(load().lc_encode_token_logprobs(ctx.h, _stream(stream), as_view(logits).ref(), _maybe(targets), scale,
+                                          _maybe(logprob), _maybe(entropy), _maybe(stats), _maybe(top_logprobs),
+                                          _maybe(top_ids)))
+
+
+def encode_token_logprobs_backward(ctx: Context, stream, logits, targets, scale, stats, d_logprob, dlogits,
+                                   entropy=None, d_entropy=None):
+    """Gradient of ``encode_token_logprobs``' logprob and entropy; ``dlogits`` may be ``logits`` itself."""
+    check(load().lc_encode_token_logprobs_backward(ctx.h, _stream(stream), as_view(logits).ref(), _maybe(targets), scale,
+                                                   as_view(stats).ref(), _maybe(entropy), _maybe(d_logprob),
+                                                   _maybe(d_entropy), as_view(dlogits).ref()))
+
+
+def encode_distill_loss(ctx: Context, stream, logits, ids, teacher, scale, loss, tail=False):
+    """Divergence of softmax(scale * logits) from a teacher's best alternatives (``ids``, ``teacher`` [..., K]):
+    renormalised, or with ``tail`` as log probabilities whose rest is one bucket."""
+    check(load().lc_encode_distill_loss(ctx.h, _stream(stream), as_view(logits).ref(), as_view(ids).ref(),
+                                        as_view(teacher).ref(), scale, int(tail), as_view(loss).ref()))
+
+
+def encode_distill_grad(ctx: Context, stream, logits, ids, teacher, scale, dlogits, d_loss=None, loss=None, tail=False):
+    """``encode_distill_loss`` (``loss`` optional) and its gradient for ``d_loss`` (1 where None) in one pass;
+    ``dlogits`` may be ``logits`` itself."""
+    check(load().lc_encode_distill_grad(ctx.h, _stream(stream), as_view(logits).ref(), as_view(ids).ref(),
+                                        as_view(teacher).ref(), scale, int(tail), _maybe(d_loss), _maybe(loss),
+                                        as_view(dlogits).ref()))
+
+
+def _waited(fn):
+    def wrapped(ctx, *args, **kwargs):
+        fn(ctx, None, *args, **kwargs)
+        ctx.sync()
+    wrapped.__name__ = fn.__name__.replace("encode_", "")
+    wrapped.__doc__ = f"``{fn.__name__}`` on the context's stream, waited for."
+    return wrapped
+
+
+token_logprobs = _waited(encode_token_logprobs)
+token_logprobs_backward = _waited(encode_token_logprobs_backward)
+distill_loss = _waited(encode_distill_loss)
+distill_grad = _waited(encode_distill_grad)
 
 
 # ---------------------------------------------------------------------------------------------

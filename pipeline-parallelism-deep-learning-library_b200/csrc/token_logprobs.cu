@@ -22,6 +22,31 @@ struct ScoreArgs {
   float scale;
 };
 
+// The token of row r, or one outside the vocabulary where none is asked for.
+__device__ __forceinline__ uint32_t token_of(const ScoreArgs& a, uint64_t r) {
+  return a.logprob.data ? static_cast<const uint32_t*>(a.targets.data)[row_at(a.g, a.targets, r)] : 0xffffffffu;
+}
+
+// What a row leaves beside the alternatives.  `xt`: the token's logit, where it is in the vocabulary.
+__device__ __forceinline__ void write_row(const ScoreArgs& a, uint64_t r, const Soft& row, float total, uint32_t token, float xt) {
+  if (a.logprob.data)
+    static_cast<float*>(a.logprob.data)[row_at(a.g, a.logprob, r)] = token < a.vocab ? logprob_of(xt, row.m, total, a.scale) : 0.0f;
+  if (a.entropy.data)
+    static_cast<float*>(a.entropy.data)[row_at(a.g, a.entropy, r)] = row.m == neg_inf() ? 0.0f : total - kLn2 * (row.t / row.s);
+  if (a.stats.data) {
+    float* st = static_cast<float*>(a.stats.data) + row_at(a.g, a.stats, r);
+    st[0] = row.m;
+    st[a.stats.inner] = total;
+  }
+}
+
+__device__ __forceinline__ void write_best(const ScoreArgs& a, uint64_t r, uint32_t k, uint64_t key, const Soft& row, float total) {
+  if (a.top_lp.data)
+    static_cast<float*>(a.top_lp.data)[row_at(a.g, a.top_lp, r) + k * a.top_lp.inner] =
+        logprob_of(value_of(key), row.m, total, a.scale);
+  if (a.top_id.data) static_cast<uint32_t*>(a.top_id.data)[row_at(a.g, a.top_id, r) + k * a.top_id.inner] = index_of(key);
+}
+
 // One block a row, every element read where its stride puts it: once for the maximum and the sums, and once more for each
 // alternative asked for.
 template <int DT>
@@ -40,19 +65,8 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_strided(ScoreArgs a) 
     const Soft row = block_merge(part, c2, red);
     const float total = logf(row.s);
     if (threadIdx.x == 0) {
-      if (a.logprob.data) {
-        const uint32_t t = static_cast<const uint32_t*>(a.targets.data)[row_at(a.g, a.targets, r)];
-        static_cast<float*>(a.logprob.data)[row_at(a.g, a.logprob, r)] =
-            t < a.vocab ? logprob_of(E::up(x[t * a.x.inner]), row.m, total, a.scale) : 0.0f;
-      }
-      if (a.entropy.data)
-        static_cast<float*>(a.entropy.data)[row_at(a.g, a.entropy, r)] =
-            row.m == neg_inf() ? 0.0f : total - kLn2 * (row.t / row.s);
-      if (a.stats.data) {
-        float* st = static_cast<float*>(a.stats.data) + row_at(a.g, a.stats, r);
-        st[0] = row.m;
-        st[a.stats.inner] = total;
-      }
+      const uint32_t t = token_of(a, r);
+      write_row(a, r, row, total, t, t < a.vocab ? E::up(x[t * a.x.inner]) : 0.0f);
     }
     uint64_t last = ~0ull;
     for (uint32_t k = 0; k < a.top; k++) {
@@ -70,16 +84,314 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_strided(ScoreArgs a) 
       __syncthreads();
       for (int w = 0; w < kThreads / 32; w++) k1 = best[w] > k1 ? best[w] : k1;
       last = k1;
-      if (threadIdx.x == 0) {
-        const uint32_t j = index_of(k1);
-        if (a.top_lp.data)
-          static_cast<float*>(a.top_lp.data)[row_at(a.g, a.top_lp, r) + k * a.top_lp.inner] =
-              logprob_of(E::up(x[j * a.x.inner]), row.m, total, a.scale);
-        if (a.top_id.data) static_cast<uint32_t*>(a.top_id.data)[row_at(a.g, a.top_id, r) + k * a.top_id.inner] = j;
-      }
+      if (threadIdx.x == 0) write_best(a, r, k, k1, row, total);
     }
     __syncthreads();
   }
+}
+
+// ---- the vocabulary as the unit axis -----------------------------------------------------------
+//
+// One cluster of blocks a row (one block where there are rows enough): each thread takes up 4 vectors of 16 bytes at a time
+// into its own running softmax; threads, blocks and the cluster merge them once at the end, in an order that does not vary.
+//
+// The alternatives come out of the same pass.  Each thread leaves the order of the largest logit of every 4 vectors (a
+// slot) in shared memory.  A bound that at least K places reach is known without looking at a place again: of the threads'
+// own largest, the q-th best of each warp, q = K over the number of warps, and of those the least.  Only slots above the
+// bound are read again (some 70 of 4096 for K = 20 of 131,072), and what lies above it is ranked by counting.
+constexpr int kMaxThreads = 512;
+constexpr int kUnroll = 4;
+constexpr uint32_t kMaxSlots = 4096;
+constexpr uint32_t kMaxKeys = 1024;
+constexpr uint32_t kMaxCluster = 8;
+
+struct Slice {  // a block's part of a row
+  const uint4* vec;    // vector 0 of the row
+  uint32_t from, to;   // its vectors
+  uint32_t head;       // places before vector 0
+  uint32_t per_slot;   // steps of kUnroll * threads vectors that share a slot
+};
+
+// Calls f(order, index) for each place of this thread's vectors in slots that reach `least`.
+template <int DT, class F>
+__device__ __forceinline__ void each_place(const Slice& sl, const uint32_t* slots, uint32_t least, F f) {
+  const uint32_t step = kUnroll * blockDim.x;
+  uint32_t b = 0;
+  for (uint32_t v0 = sl.from; v0 < sl.to; v0 += step, b++) {
+    if (slots[(b / sl.per_slot) * blockDim.x + threadIdx.x] < least) continue;
+    uint4 q[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; u++) {
+      const uint32_t v = v0 + u * blockDim.x + threadIdx.x;
+      q[u] = v < sl.to ? __ldg(sl.vec + v) : Vec<DT>::masked();
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; u++) {
+      const uint32_t v = v0 + u * blockDim.x + threadIdx.x;
+      if (v >= sl.to) break;
+      if (order_of(Vec<DT>::top(q[u])) < least) continue;
+#pragma unroll
+      for (int i = 0; i < Vec<DT>::kElems / 2; i++) {
+        const float2 x = Vec<DT>::pair(q[u], i);
+        const uint32_t j = sl.head + v * Vec<DT>::kElems + 2 * i;
+        f(order_of(x.x), j);
+        f(order_of(x.y), j + 1);
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t block_count(uint32_t v, uint32_t* red) {
+  v = __reduce_add_sync(0xffffffffu, v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x / 32] = v;
+  __syncthreads();
+  uint32_t n = 0;
+  for (uint32_t w = 0; w < blockDim.x / 32; w++) n += red[w];
+  return n;
+}
+
+// The `want` best keys of the slice in `best`, best first (fewer if it has fewer; the rest are 0).
+// `mine`: the order of the largest logit of this thread's vectors, 0 if it has none.  `edge`, `edge_at`: the order and place
+// of the logit before or behind the vectors that this thread holds, 0 if none.  `places`: how many places the slice has.
+template <int DT>
+__device__ void select(const Slice& sl, const uint32_t* slots, uint32_t mine, uint32_t edge, uint32_t edge_at, uint32_t places,
+                       uint32_t want, uint64_t* keys, uint32_t* red, uint32_t* count, uint64_t* best) {
+  const uint32_t warps = blockDim.x / 32, lane = threadIdx.x & 31;
+  const uint32_t held = min(warps, (sl.to - sl.from) / 32);  // warps whose every thread has vectors
+  const uint32_t q = held ? (want + held - 1) / held : 33;
+  for (uint32_t i = threadIdx.x; i < want; i += blockDim.x) best[i] = 0;
+  uint32_t bound = 0;
+  if (q <= 32) {
+    uint32_t left = mine;
+    for (uint32_t i = 0; i < q; i++) {
+      bound = __reduce_max_sync(0xffffffffu, left);
+      if (lane == __ffs(__ballot_sync(0xffffffffu, left == bound)) - 1) left = 0;
+    }
+  }
+  if (lane == 0) red[threadIdx.x / 32] = bound;
+  if (threadIdx.x == 0) *count = 0;
+  __syncthreads();
+  if (q <= 32) {
+    for (uint32_t w = 0; w < held; w++) bound = w == 0 ? red[0] : min(bound, red[w]);
+  }
+  want = min(want, places);
+  // Places above the bound, in any order: their keys are told apart by rank below.
+  auto collect = [&](uint32_t o, uint32_t j) {
+    if (o > bound) {
+      const uint32_t at = atomicAdd(count, 1u);
+      if (at < kMaxKeys) keys[at] = ((uint64_t)o << 32) | (0xffffffffu - j);
+    }
+  };
+  each_place<DT>(sl, slots, bound + (bound != 0xffffffffu), collect);
+  collect(edge, edge_at);
+  __syncthreads();
+  uint32_t n = *count;
+  if (n > kMaxKeys) {
+    // More than fit (a row whose best places crowd together): find the K-th largest order itself, bit by bit.  Fewer than
+    // K places lie above it.
+    uint32_t lo = bound, hi = 0xffffffffu;  // at least `want` places reach lo
+    while (lo < hi) {
+      const uint32_t mid = lo + (hi - lo) / 2 + 1;
+      uint32_t c = edge >= mid;
+      each_place<DT>(sl, slots, mid, [&](uint32_t o, uint32_t) { c += o >= mid; });
+      if (block_count(c, red) >= want) lo = mid;
+      else hi = mid - 1;
+    }
+    bound = lo;
+    __syncthreads();
+    if (threadIdx.x == 0) *count = 0;
+    __syncthreads();
+    each_place<DT>(sl, slots, bound + (bound != 0xffffffffu), collect);
+    collect(edge, edge_at);
+    __syncthreads();
+    n = *count;
+  }
+  if (n < want && bound > 0) {
+    // Places equal to the bound, from the lowest index on: the places before the vectors, the vectors in steps of one for
+    // each thread, the places behind them.
+    uint32_t have = n;
+    const uint32_t step = kUnroll * blockDim.x;
+    auto place = [&](uint32_t c, auto put) {  // c: how many this thread has
+      uint32_t incl = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t w = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= (uint32_t)o) incl += w;
+      }
+      __syncthreads();
+      if (lane == 31) red[threadIdx.x / 32] = incl;
+      __syncthreads();
+      uint32_t before = have + incl - c, all = have;
+      for (uint32_t w = 0; w < warps; w++) {
+        if (w < threadIdx.x / 32) before += red[w];
+        all += red[w];
+      }
+      put(before);
+      have = all;
+    };
+    const bool front = edge == bound && edge_at < sl.head;
+    place(front, [&](uint32_t at) {
+      if (front && at < want) keys[at] = ((uint64_t)edge << 32) | (0xffffffffu - edge_at);
+    });
+    uint32_t b = 0;
+    for (uint32_t v0 = sl.from; v0 < sl.to && have < want; v0 += step, b++) {
+      const bool may = slots[(b / sl.per_slot) * blockDim.x + threadIdx.x] >= bound;
+      for (int u = 0; u < kUnroll && have < want; u++) {
+        const uint32_t v = v0 + u * blockDim.x + threadIdx.x;
+        uint32_t hits = 0;
+        if (may && v < sl.to) {
+          const uint4 x = __ldg(sl.vec + v);
+#pragma unroll
+          for (int i = 0; i < Vec<DT>::kElems / 2; i++) {
+            const float2 p = Vec<DT>::pair(x, i);
+            hits |= (uint32_t)(order_of(p.x) == bound) << (2 * i) | (uint32_t)(order_of(p.y) == bound) << (2 * i + 1);
+          }
+        }
+        place(__popc(hits), [&](uint32_t at) {
+          for (; hits && at < want; hits &= hits - 1, at++)
+            keys[at] = ((uint64_t)bound << 32) | (0xffffffffu - (sl.head + v * Vec<DT>::kElems + (__ffs(hits) - 1)));
+        });
+      }
+    }
+    if (have < want) {
+      const bool back = edge == bound && edge_at >= sl.head;
+      place(back, [&](uint32_t at) {
+        if (back && at < want) keys[at] = ((uint64_t)edge << 32) | (0xffffffffu - edge_at);
+      });
+    }
+    __syncthreads();
+    n = min(have, want);
+  }
+  for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
+    const uint64_t key = keys[i];
+    uint32_t rank = 0;
+    for (uint32_t o = 0; o < n; o++) rank += keys[o] > key;
+    if (rank < want) best[rank] = key;
+  }
+  __syncthreads();
+}
+
+template <int DT, bool SUM_T, bool TOP>
+__global__ void __launch_bounds__(kMaxThreads, 2) token_logprobs_rows(ScoreArgs a, uint32_t cluster, uint32_t per_slot) {
+  using E = Elem<DT>;
+  constexpr uint32_t kE = Vec<DT>::kElems;
+  extern __shared__ uint64_t dyn[];
+  __shared__ Soft red[kMaxThreads / 32];
+  __shared__ Soft parts[kMaxCluster];
+  __shared__ uint32_t red_u[kMaxThreads / 32];
+  __shared__ uint32_t count;
+  uint64_t* keys = dyn;                                          // [kMaxKeys]
+  uint64_t* best = keys + kMaxKeys;                              // [top]
+  uint64_t* lists = best + a.top;                                // [cluster][top]: the blocks' best, in block 0
+  uint32_t* slots = reinterpret_cast<uint32_t*>(lists + (cluster > 1 ? cluster * a.top : 0));  // [n_slots][threads]
+  const uint32_t rank = cluster > 1 ? cluster_rank() : 0;
+  const float c2 = a.scale * kLog2e;
+  // Cluster barriers alternate: block 0's buffers are free (at first: it has started), and all blocks' parts are in them.
+  if (cluster > 1) cluster_arrive();
+  for (uint64_t r = blockIdx.x / cluster; r < a.g.rows; r += gridDim.x / cluster) {
+    const typename E::T* x = static_cast<const typename E::T*>(a.x.data) + row_at(a.g, a.x, r);
+    const Span span = span_of<DT>(x, a.vocab);
+    Slice sl;
+    sl.vec = reinterpret_cast<const uint4*>(x + span.head);
+    sl.head = span.head;
+    sl.per_slot = per_slot;
+    const uint32_t share = ((span.vecs + cluster - 1) / cluster + 31) / 32 * 32;
+    sl.from = min(span.vecs, rank * share);
+    sl.to = min(span.vecs, sl.from + share);
+    // block 0 has the places before the vectors (threads 0-7) and behind them (8-15), and the token
+    float edge = neg_inf(), xt = 0.0f;
+    uint32_t edge_at = 0xffffffffu, token = 0xffffffffu;
+    if (rank == 0 && threadIdx.x < 16) {
+      const uint32_t i = threadIdx.x & 7;
+      if (threadIdx.x < 8 ? i < span.head : i < span.tail) {
+        edge_at = threadIdx.x < 8 ? i : span.head + span.vecs * kE + i;
+        edge = E::up(x[edge_at]);
+      }
+      if (threadIdx.x == 0) {
+        token = token_of(a, r);
+        if (token < a.vocab) xt = E::up(x[token]);
+      }
+    }
+    Run run{neg_inf(), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+    uint32_t mine = 0, slot = 0, in_slot = 0;
+    uint32_t* next = slots + threadIdx.x;
+    for (uint32_t v0 = sl.from; v0 < sl.to; v0 += kUnroll * blockDim.x) {
+      uint4 q[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; u++) {
+        const uint32_t v = v0 + u * blockDim.x + threadIdx.x;
+        q[u] = v < sl.to ? load_once(sl.vec + v) : Vec<DT>::masked();
+      }
+      float top = Vec<DT>::top(q[0]);
+#pragma unroll
+      for (int u = 1; u < kUnroll; u++) top = max_nan(top, Vec<DT>::top(q[u]));
+      take<DT, kUnroll, SUM_T>(run, q, top, c2);
+      if constexpr (TOP) {
+        slot = max(slot, v0 + threadIdx.x < sl.to ? order_of(top) : 0u);
+        mine = max(mine, slot);
+        if (++in_slot == per_slot || v0 + kUnroll * blockDim.x >= sl.to) {
+          *next = slot;
+          next += blockDim.x;
+          slot = in_slot = 0;
+        }
+      }
+    }
+    Soft part{run.m, run.s.x + run.s.y, run.t.x + run.t.y};
+    if (edge_at != 0xffffffffu) part = merge(part, Soft{edge, edge == neg_inf() ? 0.0f : 1.0f, 0.0f}, c2);
+    Soft row = block_merge(part, c2, red);
+    if constexpr (TOP) {
+      const uint32_t places = (sl.to - sl.from) * kE + (rank == 0 ? span.head + span.tail : 0);
+      select<DT>(sl, slots, mine, edge_at != 0xffffffffu ? order_of(edge) : 0, edge_at, places, a.top, keys, red_u, &count, best);
+    }
+    if (cluster > 1) {
+      cluster_wait();
+      if (threadIdx.x == 0) {
+        const uint32_t at = remote(&parts[rank], 0);
+        store_remote(at, row.m);
+        store_remote(at + 4, row.s);
+        store_remote(at + 8, row.t);
+      }
+      if constexpr (TOP) {
+        for (uint32_t i = threadIdx.x; i < a.top; i += blockDim.x) store_remote(remote(lists + rank * a.top + i, 0), best[i]);
+      }
+      cluster_arrive();
+      cluster_wait();
+    }
+    if (rank == 0) {
+      if (cluster > 1) {
+        row = parts[0];
+        for (uint32_t c = 1; c < cluster; c++) row = merge(row, parts[c], c2);
+      }
+      const float total = logf(row.s);
+      if (threadIdx.x == 0) write_row(a, r, row, total, token, xt);
+      if constexpr (TOP) {
+        if (cluster == 1) {
+          for (uint32_t k = threadIdx.x; k < a.top; k += blockDim.x) write_best(a, r, k, best[k], row, total);
+        } else {
+          // the K best of the blocks' lists, each of them in order: a key's rank is how many are better in every list
+          for (uint32_t i = threadIdx.x; i < cluster * a.top; i += blockDim.x) {
+            const uint64_t key = lists[i];
+            uint32_t k = key ? 0 : a.top;
+            for (uint32_t c = 0; c < cluster && k < a.top; c++) {
+              const uint64_t* list = lists + c * a.top;
+              uint32_t lo = 0, hi = a.top;
+              while (lo < hi) {
+                const uint32_t mid = (lo + hi) / 2;
+                if (list[mid] > key) lo = mid + 1;
+                else hi = mid;
+              }
+              k += lo;
+            }
+            if (k < a.top) write_best(a, r, k, key, row, total);
+          }
+        }
+      }
+    }
+    if (cluster > 1) cluster_arrive();
+    __syncthreads();
+  }
+  if (cluster > 1) cluster_wait();
 }
 
 struct GradArgs {
@@ -155,6 +467,52 @@ lc_status launched(lc_context* ctx, const char* name) {
 
 bool good_scale(float s) { return std::isfinite(s) && s > 0.0f; }
 
+// How a row is spread: blocks of `threads` in a cluster of `cluster`, and the slots of its alternatives.
+struct Spread {
+  uint32_t cluster, threads, n_slots, per_slot;
+  size_t shared;
+};
+
+// Enough blocks to fill the device, as long as each has 2 steps of 512 threads left to do: one row of 131,072 bf16 over 8
+// blocks.  From 2 rows an SM on, one block a row.  A block has the threads that its vectors keep busy at 4 each, and 2 for
+// each alternative asked for, so that the bound on them (select) comes from several warps.
+Spread spread_of(const lc_context* ctx, uint64_t rows, uint64_t vocab, uint32_t elems, uint32_t top) {
+  Spread s{};
+  const uint64_t vecs = vocab / elems;
+  s.cluster = 1;
+  while (s.cluster < kMaxCluster && rows * s.cluster < 2ull * ctx->sm_count && vecs / (2 * s.cluster) >= 2ull * kUnroll * 256)
+    s.cluster *= 2;
+  const uint64_t share = std::max<uint64_t>(((vecs + s.cluster - 1) / s.cluster + 31) / 32 * 32, 1);
+  const uint64_t busy = std::max<uint64_t>((share + kUnroll - 1) / kUnroll, 2 * top);
+  s.threads = (uint32_t)std::min<uint64_t>(kMaxThreads, (busy + 31) / 32 * 32);
+  const uint64_t steps = (share + (uint64_t)kUnroll * s.threads - 1) / ((uint64_t)kUnroll * s.threads);
+  const uint64_t rows_of_slots = std::max<uint64_t>(1, kMaxSlots / s.threads);
+  s.per_slot = (uint32_t)((steps + rows_of_slots - 1) / rows_of_slots);
+  s.n_slots = (uint32_t)((steps + s.per_slot - 1) / s.per_slot);
+  if (top) s.shared = sizeof(uint64_t) * (kMaxKeys + top + (s.cluster > 1 ? s.cluster * top : 0)) + sizeof(uint32_t) * s.n_slots * s.threads;
+  return s;
+}
+
+template <int DT>
+cudaError_t launch_rows(const lc_context* ctx, const ScoreArgs& a, cudaStream_t stream) {
+  const Spread s = spread_of(ctx, a.g.rows, a.vocab, Vec<DT>::kElems, a.top);
+  void (*kernel)(ScoreArgs, uint32_t, uint32_t) =
+      a.top ? (a.entropy.data ? token_logprobs_rows<DT, true, true> : token_logprobs_rows<DT, false, true>)
+            : (a.entropy.data ? token_logprobs_rows<DT, true, false> : token_logprobs_rows<DT, false, false>);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(std::min<uint64_t>(a.g.rows, kMaxGrid) * s.cluster));
+  cfg.blockDim = dim3(s.threads);
+  cfg.dynamicSmemBytes = s.shared;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = s.cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = s.cluster > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, a, s.cluster, s.per_slot);
+}
+
 unsigned row_grid(uint64_t rows) { return (unsigned)std::min<uint64_t>(rows, kMaxGrid); }
 
 }  // namespace
@@ -204,6 +562,12 @@ lc_status lc_encode_token_logprobs(lc_context* ctx, void* stream, const lc_view*
   a.scale = scale;
   DeviceGuard on(ctx->device);
   cudaStream_t s = stream_of(ctx, stream);
+  if (a.x.inner == 1 || a.vocab == 1) {
+    cudaError_t e = logits->dtype == LC_F32 ? launch_rows<LC_F32>(ctx, a, s)
+                    : logits->dtype == LC_F16 ? launch_rows<LC_F16>(ctx, a, s) : launch_rows<LC_BF16>(ctx, a, s);
+    if (e != cudaSuccess) return cuda_fail(e, "token_logprobs_rows");
+    return launched(ctx, "token_logprobs_rows");
+  }
   const unsigned grid = row_grid(a.g.rows);
   if (logits->dtype == LC_F32) token_logprobs_strided<LC_F32><<<grid, kThreads, 0, s>>>(a);
   else if (logits->dtype == LC_F16) token_logprobs_strided<LC_F16><<<grid, kThreads, 0, s>>>(a);

@@ -99,10 +99,14 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_strided(ScoreArgs a) 
 // slot) in shared memory.  A bound that at least K places reach is known without looking at a place again: of the threads'
 // own largest, the q-th best of each warp, q = K over the number of warps, and of those the least.  Only slots above the
 // bound are read again (some 70 of 4096 for K = 20 of 131,072), and what lies above it is ranked by counting.
-constexpr int kMaxThreads = 512;
-constexpr int kUnroll = 4;
+constexpr int kMaxThreads = 256;
+template <int DT>
+constexpr int kUnroll = 32 / Vec<DT>::kElems;  // vectors of a step: 32 places a thread
+template <int DT>
+constexpr int kResident = DT == LC_F32 ? 5 : 6;  // blocks an SM
 constexpr uint32_t kMaxSlots = 4096;
-constexpr uint32_t kMaxKeys = 1024;
+constexpr uint32_t kMaxKeys = 512;
+constexpr uint32_t kMaxRead = 256;  // slots that are read again in one go
 constexpr uint32_t kMaxCluster = 8;
 
 struct Slice {  // a block's part of a row
@@ -115,18 +119,19 @@ struct Slice {  // a block's part of a row
 // Calls f(order, index) for each place of this thread's vectors in slots that reach `least`.
 template <int DT, class F>
 __device__ __forceinline__ void each_place(const Slice& sl, const uint32_t* slots, uint32_t least, F f) {
-  const uint32_t step = kUnroll * blockDim.x;
+  constexpr int kSteps = kUnroll<DT>;
+  const uint32_t step = kSteps * blockDim.x;
   uint32_t b = 0;
   for (uint32_t v0 = sl.from; v0 < sl.to; v0 += step, b++) {
     if (slots[(b / sl.per_slot) * blockDim.x + threadIdx.x] < least) continue;
-    uint4 q[kUnroll];
+    uint4 q[kSteps];
 #pragma unroll
-    for (int u = 0; u < kUnroll; u++) {
+    for (int u = 0; u < kSteps; u++) {
       const uint32_t v = v0 + u * blockDim.x + threadIdx.x;
       q[u] = v < sl.to ? __ldg(sl.vec + v) : Vec<DT>::masked();
     }
 #pragma unroll
-    for (int u = 0; u < kUnroll; u++) {
+    for (int u = 0; u < kSteps; u++) {
       const uint32_t v = v0 + u * blockDim.x + threadIdx.x;
       if (v >= sl.to) break;
       if (order_of(Vec<DT>::top(q[u])) < least) continue;
@@ -151,12 +156,23 @@ __device__ __forceinline__ uint32_t block_count(uint32_t v, uint32_t* red) {
   return n;
 }
 
+// Shared memory of select.
+struct Work {
+  uint64_t* keys;   // [kMaxKeys]
+  uint32_t* read;   // [kMaxRead]
+  uint32_t* red;    // one for each warp
+  uint32_t* count;  // 2
+};
+
 // The `want` best keys of the slice in `best`, best first (fewer if it has fewer; the rest are 0).
 // `mine`: the order of the largest logit of this thread's vectors, 0 if it has none.  `edge`, `edge_at`: the order and place
 // of the logit before or behind the vectors that this thread holds, 0 if none.  `places`: how many places the slice has.
 template <int DT>
 __device__ void select(const Slice& sl, const uint32_t* slots, uint32_t mine, uint32_t edge, uint32_t edge_at, uint32_t places,
-                       uint32_t want, uint64_t* keys, uint32_t* red, uint32_t* count, uint64_t* best) {
+                       uint32_t want, const Work& w, uint64_t* best) {
+  constexpr int kSteps = kUnroll<DT>;
+  uint64_t* keys = w.keys;
+  uint32_t *red = w.red, *count = w.count;
   const uint32_t warps = blockDim.x / 32, lane = threadIdx.x & 31;
   const uint32_t held = min(warps, (sl.to - sl.from) / 32);  // warps whose every thread has vectors
   const uint32_t q = held ? (want + held - 1) / held : 33;
@@ -170,10 +186,10 @@ __device__ void select(const Slice& sl, const uint32_t* slots, uint32_t mine, ui
     }
   }
   if (lane == 0) red[threadIdx.x / 32] = bound;
-  if (threadIdx.x == 0) *count = 0;
+  if (threadIdx.x == 0) count[0] = count[1] = 0;
   __syncthreads();
   if (q <= 32) {
-    for (uint32_t w = 0; w < held; w++) bound = w == 0 ? red[0] : min(bound, red[w]);
+    for (uint32_t i = 0; i < held; i++) bound = i == 0 ? red[0] : min(bound, red[i]);
   }
   want = min(want, places);
   // Places above the bound, in any order: their keys are told apart by rank below.
@@ -183,8 +199,35 @@ __device__ void select(const Slice& sl, const uint32_t* slots, uint32_t mine, ui
       if (at < kMaxKeys) keys[at] = ((uint64_t)o << 32) | (0xffffffffu - j);
     }
   };
-  each_place<DT>(sl, slots, bound + (bound != 0xffffffffu), collect);
+  // The slots above the bound go to a list first, so that all their vectors are on the way at once.
+  const uint32_t step = kSteps * blockDim.x, steps = (sl.to - sl.from + step - 1) / step;
+  const uint32_t rows_of_slots = (steps + sl.per_slot - 1) / sl.per_slot;
+  for (uint32_t i = 0; i < rows_of_slots; i++)
+    if (slots[i * blockDim.x + threadIdx.x] > bound) {
+      const uint32_t at = atomicAdd(count + 1, 1u);
+      if (at < kMaxRead) w.read[at] = i << 16 | threadIdx.x;
+    }
   collect(edge, edge_at);
+  __syncthreads();
+  const uint32_t reads = count[1], per = sl.per_slot * kSteps;
+  if (reads <= kMaxRead) {
+    for (uint32_t i = threadIdx.x; i < reads * per; i += blockDim.x) {
+      const uint32_t e = w.read[i / per], k = i % per;
+      const uint32_t v = sl.from + ((e >> 16) * per + k) * blockDim.x + (e & 0xffffu);
+      if (v >= sl.to) continue;
+      const uint4 q = __ldg(sl.vec + v);
+      if (order_of(Vec<DT>::top(q)) <= bound) continue;
+#pragma unroll
+      for (int i2 = 0; i2 < Vec<DT>::kElems / 2; i2++) {
+        const float2 x = Vec<DT>::pair(q, i2);
+        const uint32_t j = sl.head + v * Vec<DT>::kElems + 2 * i2;
+        collect(order_of(x.x), j);
+        collect(order_of(x.y), j + 1);
+      }
+    }
+  } else {
+    each_place<DT>(sl, slots, bound + (bound != 0xffffffffu), collect);
+  }
   __syncthreads();
   uint32_t n = *count;
   if (n > kMaxKeys) {
@@ -211,21 +254,20 @@ __device__ void select(const Slice& sl, const uint32_t* slots, uint32_t mine, ui
     // Places equal to the bound, from the lowest index on: the places before the vectors, the vectors in steps of one for
     // each thread, the places behind them.
     uint32_t have = n;
-    const uint32_t step = kUnroll * blockDim.x;
     auto place = [&](uint32_t c, auto put) {  // c: how many this thread has
       uint32_t incl = c;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t w = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= (uint32_t)o) incl += w;
+        const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= (uint32_t)o) incl += up;
       }
       __syncthreads();
       if (lane == 31) red[threadIdx.x / 32] = incl;
       __syncthreads();
       uint32_t before = have + incl - c, all = have;
-      for (uint32_t w = 0; w < warps; w++) {
-        if (w < threadIdx.x / 32) before += red[w];
-        all += red[w];
+      for (uint32_t i = 0; i < warps; i++) {
+        if (i < threadIdx.x / 32) before += red[i];
+        all += red[i];
       }
       put(before);
       have = all;
@@ -237,7 +279,7 @@ __device__ void select(const Slice& sl, const uint32_t* slots, uint32_t mine, ui
     uint32_t b = 0;
     for (uint32_t v0 = sl.from; v0 < sl.to && have < want; v0 += step, b++) {
       const bool may = slots[(b / sl.per_slot) * blockDim.x + threadIdx.x] >= bound;
-      for (int u = 0; u < kUnroll && have < want; u++) {
+      for (int u = 0; u < kSteps && have < want; u++) {
         const uint32_t v = v0 + u * blockDim.x + threadIdx.x;
         uint32_t hits = 0;
         if (may && v < sl.to) {
@@ -266,6 +308,7 @@ __device__ void select(const Slice& sl, const uint32_t* slots, uint32_t mine, ui
   for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
     const uint64_t key = keys[i];
     uint32_t rank = 0;
+#pragma unroll 8
     for (uint32_t o = 0; o < n; o++) rank += keys[o] > key;
     if (rank < want) best[rank] = key;
   }
@@ -273,16 +316,16 @@ __device__ void select(const Slice& sl, const uint32_t* slots, uint32_t mine, ui
 }
 
 template <int DT, bool SUM_T, bool TOP>
-__global__ void __launch_bounds__(kMaxThreads, 2) token_logprobs_rows(ScoreArgs a, uint32_t cluster, uint32_t per_slot) {
+__global__ void __launch_bounds__(kMaxThreads, kResident<DT>) token_logprobs_rows(ScoreArgs a, uint32_t cluster, uint32_t per_slot) {
   using E = Elem<DT>;
   constexpr uint32_t kE = Vec<DT>::kElems;
+  constexpr int kSteps = kUnroll<DT>;
   extern __shared__ uint64_t dyn[];
   __shared__ Soft red[kMaxThreads / 32];
   __shared__ Soft parts[kMaxCluster];
-  __shared__ uint32_t red_u[kMaxThreads / 32];
-  __shared__ uint32_t count;
-  uint64_t* keys = dyn;                                          // [kMaxKeys]
-  uint64_t* best = keys + kMaxKeys;                              // [top]
+  __shared__ uint32_t read[kMaxRead], red_u[kMaxThreads / 32], count[2];
+  const Work work{dyn, read, red_u, count};
+  uint64_t* best = dyn + kMaxKeys;                               // [top]
   uint64_t* lists = best + a.top;                                // [cluster][top]: the blocks' best, in block 0
   uint32_t* slots = reinterpret_cast<uint32_t*>(lists + (cluster > 1 ? cluster * a.top : 0));  // [n_slots][threads]
   const uint32_t rank = cluster > 1 ? cluster_rank() : 0;
@@ -313,36 +356,60 @@ __global__ void __launch_bounds__(kMaxThreads, 2) token_logprobs_rows(ScoreArgs 
         if (token < a.vocab) xt = E::up(x[token]);
       }
     }
-    Run run{neg_inf(), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+    Run run = empty_run();
     uint32_t mine = 0, slot = 0, in_slot = 0;
     uint32_t* next = slots + threadIdx.x;
-    for (uint32_t v0 = sl.from; v0 < sl.to; v0 += kUnroll * blockDim.x) {
-      uint4 q[kUnroll];
-#pragma unroll
-      for (int u = 0; u < kUnroll; u++) {
-        const uint32_t v = v0 + u * blockDim.x + threadIdx.x;
-        q[u] = v < sl.to ? load_once(sl.vec + v) : Vec<DT>::masked();
+    auto leave = [&](float top, bool last) {  // the largest of a step's logits goes to its slot
+      slot = max(slot, order_of(top));
+      if (++in_slot == per_slot || last) {
+        mine = max(mine, slot);
+        *next = slot;
+        next += blockDim.x;
+        slot = in_slot = 0;
       }
+    };
+    const uint32_t step = kSteps * blockDim.x;
+    uint32_t v0 = sl.from;
+    for (; v0 + step <= sl.to; v0 += step) {
+      uint4 q[kSteps];
+#pragma unroll
+      for (int u = 0; u < kSteps; u++) q[u] = load_once(sl.vec + v0 + u * blockDim.x + threadIdx.x);
       float top = Vec<DT>::top(q[0]);
 #pragma unroll
-      for (int u = 1; u < kUnroll; u++) top = max_nan(top, Vec<DT>::top(q[u]));
-      take<DT, kUnroll, SUM_T>(run, q, top, c2);
+      for (int u = 1; u < kSteps; u++) top = max_nan(top, Vec<DT>::top(q[u]));
+      take<DT, kSteps, SUM_T>(run, q, top, c2);
+      if constexpr (TOP) leave(top, v0 + step >= sl.to);
+    }
+    if (v0 < sl.to) {
+      uint4 q[kSteps][1];
+#pragma unroll
+      for (int u = 0; u < kSteps; u++) {
+        const uint32_t v = v0 + u * blockDim.x + threadIdx.x;
+        if (v < sl.to) q[u][0] = load_once(sl.vec + v);
+      }
+      float top = neg_inf();
+#pragma unroll
+      for (int u = 0; u < kSteps; u++) {
+        if (v0 + u * blockDim.x + threadIdx.x >= sl.to) break;
+        const float t = Vec<DT>::top(q[u][0]);
+        top = max_nan(top, t);
+        take<DT, 1, SUM_T>(run, q[u], t, c2);
+      }
       if constexpr (TOP) {
-        slot = max(slot, v0 + threadIdx.x < sl.to ? order_of(top) : 0u);
-        mine = max(mine, slot);
-        if (++in_slot == per_slot || v0 + kUnroll * blockDim.x >= sl.to) {
+        if (v0 + threadIdx.x < sl.to) {
+          leave(top, true);
+        } else {  // nothing of this step is this thread's
+          mine = max(mine, slot);
           *next = slot;
-          next += blockDim.x;
-          slot = in_slot = 0;
         }
       }
     }
-    Soft part{run.m, run.s.x + run.s.y, run.t.x + run.t.y};
+    Soft part = soft_of(run, c2);
     if (edge_at != 0xffffffffu) part = merge(part, Soft{edge, edge == neg_inf() ? 0.0f : 1.0f, 0.0f}, c2);
     Soft row = block_merge(part, c2, red);
     if constexpr (TOP) {
       const uint32_t places = (sl.to - sl.from) * kE + (rank == 0 ? span.head + span.tail : 0);
-      select<DT>(sl, slots, mine, edge_at != 0xffffffffu ? order_of(edge) : 0, edge_at, places, a.top, keys, red_u, &count, best);
+      select<DT>(sl, slots, mine, edge_at != 0xffffffffu ? order_of(edge) : 0, edge_at, places, a.top, work, best);
     }
     if (cluster > 1) {
       cluster_wait();
@@ -476,16 +543,20 @@ struct Spread {
 // Enough blocks to fill the device, as long as each has 2 steps of 512 threads left to do: one row of 131,072 bf16 over 8
 // blocks.  From 2 rows an SM on, one block a row.  A block has the threads that its vectors keep busy at 4 each, and 2 for
 // each alternative asked for, so that the bound on them (select) comes from several warps.
-Spread spread_of(const lc_context* ctx, uint64_t rows, uint64_t vocab, uint32_t elems, uint32_t top) {
+Spread spread_of(const lc_context* ctx, uint64_t rows, uint64_t vocab, uint32_t elems, uint32_t unroll, uint32_t top) {
   Spread s{};
   const uint64_t vecs = vocab / elems;
   s.cluster = 1;
-  while (s.cluster < kMaxCluster && rows * s.cluster < 2ull * ctx->sm_count && vecs / (2 * s.cluster) >= 2ull * kUnroll * 256)
+  while (s.cluster < kMaxCluster && rows * s.cluster < 2ull * ctx->sm_count && vecs / (2 * s.cluster) >= 2ull * unroll * 256)
     s.cluster *= 2;
   const uint64_t share = std::max<uint64_t>(((vecs + s.cluster - 1) / s.cluster + 31) / 32 * 32, 1);
-  const uint64_t busy = std::max<uint64_t>((share + kUnroll - 1) / kUnroll, 2 * top);
+  const uint64_t busy = std::max<uint64_t>((share + unroll - 1) / unroll, 2 * top);
   s.threads = (uint32_t)std::min<uint64_t>(kMaxThreads, (busy + 31) / 32 * 32);
-  const uint64_t steps = (share + (uint64_t)kUnroll * s.threads - 1) / ((uint64_t)kUnroll * s.threads);
+  if (busy > kMaxThreads) {  // several steps: of one length, so that the last one is not nearly empty
+    const uint64_t n = (busy + kMaxThreads - 1) / kMaxThreads;
+    s.threads = (uint32_t)(((busy + n - 1) / n + 31) / 32 * 32);
+  }
+  const uint64_t steps = (share + (uint64_t)unroll * s.threads - 1) / ((uint64_t)unroll * s.threads);
   const uint64_t rows_of_slots = std::max<uint64_t>(1, kMaxSlots / s.threads);
   s.per_slot = (uint32_t)((steps + rows_of_slots - 1) / rows_of_slots);
   s.n_slots = (uint32_t)((steps + s.per_slot - 1) / s.per_slot);
@@ -495,7 +566,7 @@ Spread spread_of(const lc_context* ctx, uint64_t rows, uint64_t vocab, uint32_t 
 
 template <int DT>
 cudaError_t launch_rows(const lc_context* ctx, const ScoreArgs& a, cudaStream_t stream) {
-  const Spread s = spread_of(ctx, a.g.rows, a.vocab, Vec<DT>::kElems, a.top);
+  const Spread s = spread_of(ctx, a.g.rows, a.vocab, Vec<DT>::kElems, kUnroll<DT>, a.top);
   void (*kernel)(ScoreArgs, uint32_t, uint32_t) =
       a.top ? (a.entropy.data ? token_logprobs_rows<DT, true, true> : token_logprobs_rows<DT, false, true>)
             : (a.entropy.data ? token_logprobs_rows<DT, true, false> : token_logprobs_rows<DT, false, false>);

@@ -75,26 +75,6 @@ __device__ __forceinline__ uint64_t row_at(const Rows& g, const RowOperand& o, u
 
 // ---- 16 bytes of a row at a time -------------------------------------------------------------
 
-// two f32 operations in one instruction
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
-      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
-      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
-      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
-      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // 16 bytes of logits as pairs of f32, their largest (NaN if any is), and pairs of f32 rounded back
@@ -114,6 +94,11 @@ struct Vec {  // 16-bit types
     return *reinterpret_cast<const uint32_t*>(&w);
   }
   static __device__ __forceinline__ float2 pair(const uint4& q, int i) { return up(i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w); }
+  static __device__ __forceinline__ float2 pair_bounded(const uint4& q, int i) {  // bf16: no place below -1e30
+    const uint32_t low = 0xf149f149u;
+    const T2 w = __hmax2_nan(word(i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w), word(low));
+    return up(*reinterpret_cast<const uint32_t*>(&w));
+  }
   static __device__ __forceinline__ float top(const uint4& q) {
     const T2 m = __hmax2_nan(__hmax2_nan(word(q.x), word(q.y)), __hmax2_nan(word(q.z), word(q.w)));
     const float2 f = up(*reinterpret_cast<const uint32_t*>(&m));
@@ -167,53 +152,105 @@ __device__ __forceinline__ Soft merge(const Soft& a, const Soft& b, float c2) {
   return r;
 }
 
-__device__ __forceinline__ Soft warp_merge(Soft v, float c2) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Soft w{__shfl_xor_sync(0xffffffffu, v.m, o), __shfl_xor_sync(0xffffffffu, v.s, o), __shfl_xor_sync(0xffffffffu, v.t, o)};
-    // the same operand order on both sides, so that every lane holds the same bits
-    v = (threadIdx.x & o) ? merge(w, v, c2) : merge(v, w, c2);
-  }
-  return v;
+// The larger of a warp's values, or NaN if any is.
+__device__ __forceinline__ float warp_top(float v) {
+  float y;
+  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(v));
+  return y;
 }
 
-// The whole block's part of the row, in every thread.  `red`: one entry for each warp.  Ends with a barrier before `red`
-// may be written again only if the caller has one.
+// A warp's parts, in every lane: moved to the common maximum first, then summed in a tree that is the same for all lanes.
+__device__ __forceinline__ Soft warp_merge(Soft v, float c2) {
+  const float m = warp_top(v.m);
+  const float u = v.m == neg_inf() ? 0.0f : max_nan((v.m - base_of(m)) * c2, kFar), f = ex2(u);
+  float s = v.s * f, t = f * (v.t + u * v.s);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    t += __shfl_xor_sync(0xffffffffu, t, o);
+  }
+  return Soft{m, s, t};
+}
+
+// The whole block's part of the row, in every thread.  `red`: one entry for each warp, of at most 32; the caller keeps a
+// barrier between two uses.
 __device__ __forceinline__ Soft block_merge(Soft v, float c2, Soft* red) {
   v = warp_merge(v, c2);
-  const int warps = blockDim.x / 32;  // at most 32
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x / 32] = v;
+  const uint32_t warps = blockDim.x / 32, lane = threadIdx.x & 31;
+  if (lane == 0) red[threadIdx.x / 32] = v;
   __syncthreads();
-  Soft w = (int)(threadIdx.x & 31) < warps ? red[threadIdx.x & 31] : Soft{neg_inf(), 0.0f, 0.0f};
-  return warp_merge(w, c2);
+  return warp_merge(lane < warps ? red[lane] : Soft{neg_inf(), 0.0f, 0.0f}, c2);
 }
 
 // The softmax of what one thread has seen, in two lanes of sums.
+//
+// While the largest logit is of an ordinary size, d is one fused multiply-add, x c2 - mc, against mc = m c2 as it rounds:
+// one rounding a place, as good as (x - m) c2 with its two.  The sums then stand against mc / c2 and not m; soft_of moves
+// them by the difference.  Logits beyond kWide, where x c2 could overflow or places could not be told from masked ones, and
+// scales far from 1 take (x - m) c2.
 struct Run {
-  float m;
+  float m, mc;
   float2 s, t;
 };
+constexpr float kWide = 1e25f;
+__device__ __forceinline__ Run empty_run() { return Run{neg_inf(), 0.0f, make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)}; }
+// NaN and the infinities are wide
+__device__ __forceinline__ bool is_wide(float m, float c2) { return !(fabsf(m) < kWide) || !(c2 > 1e-3f && c2 < 1e4f); }
 
 // Takes up N vectors whose largest logit is `top`.  SUM_T: with the sum that the entropy needs.
 template <int DT, int N, bool SUM_T>
 __device__ __forceinline__ void take(Run& r, const uint4 (&q)[N], float top, float c2) {
   const float m = max_nan(r.m, top);
+  const bool wide = is_wide(m, c2);
   if (!(m == r.m)) {  // a new largest logit (or a NaN): seldom, after the first vectors of a row
-    const float u = r.m == neg_inf() ? 0.0f : max_nan((r.m - base_of(m)) * c2, kFar), f = ex2(u);
-    if constexpr (SUM_T) r.t = mul2(both(f), fma2(both(u), r.s, r.t));
-    r.s = mul2(both(f), r.s);
+    const float mc = wide ? 0.0f : m * c2;
+    float u = wide || is_wide(r.m, c2) ? (r.m - base_of(m)) * c2 : r.mc - mc;
+    u = r.m == neg_inf() ? 0.0f : max_nan(u, kFar);
+    const float2 f = both(ex2(u));
+    if constexpr (SUM_T) r.t = __fmul2_rn(f, __ffma2_rn(both(u), r.s, r.t));
+    r.s = __fmul2_rn(f, r.s);
     r.m = m;
+    r.mc = mc;
   }
-  const float2 minus = both(-base_of(r.m)), c = both(c2);
+  const float2 c = both(c2);
+  if (!wide) {
+    const float2 minus = both(-r.mc);
+#pragma unroll
+    for (int n = 0; n < N; n++)
+#pragma unroll
+      for (int i = 0; i < Vec<DT>::kElems / 2; i++) {
+        // a masked place must not give -inf * 0 in the product below: bf16 is bounded before it is widened, two places at a
+        // time (-1e30 has weight 0 against an m of ordinary size), the other types behind
+        float2 x;
+        if constexpr (DT == LC_BF16 && SUM_T) x = Vec<DT>::pair_bounded(q[n], i);
+        else x = Vec<DT>::pair(q[n], i);
+        float2 d = __ffma2_rn(x, c, minus);
+        const float2 e = make_float2(ex2(d.x), ex2(d.y));
+        r.s = __fadd2_rn(r.s, e);
+        if constexpr (SUM_T) {
+          if constexpr (DT != LC_BF16) d = make_float2(max_nan(d.x, kFar), max_nan(d.y, kFar));
+          r.t = __ffma2_rn(e, d, r.t);
+        }
+      }
+    return;
+  }
+  const float2 minus = both(-base_of(r.m));
 #pragma unroll
   for (int n = 0; n < N; n++)
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < Vec<DT>::kElems / 2; i++) {
-      float2 d = mul2(add2(Vec<DT>::pair(q[n], i), minus), c);
+      const float2 d = __fmul2_rn(__fadd2_rn(Vec<DT>::pair(q[n], i), minus), c);
       const float2 e = make_float2(ex2(d.x), ex2(d.y));
-      r.s = add2(r.s, e);
-      if constexpr (SUM_T) r.t = fma2(e, make_float2(max_nan(d.x, kFar), max_nan(d.y, kFar)), r.t);
+      r.s = __fadd2_rn(r.s, e);
+      if constexpr (SUM_T) r.t = __ffma2_rn(e, make_float2(max_nan(d.x, kFar), max_nan(d.y, kFar)), r.t);
     }
+}
+
+__device__ __forceinline__ Soft soft_of(const Run& r, float c2) {
+  const float s = r.s.x + r.s.y, t = r.t.x + r.t.y;
+  if (is_wide(r.m, c2)) return Soft{r.m, s, t};
+  const float off = __fmaf_rn(r.m, c2, -r.mc), f = ex2(-off);  // m c2 - mc
+  return Soft{r.m, s * f, f * (t - off * s)};
 }
 
 // Order of the alternatives: by value, NaN above all, the two zeros equal; equal values by the lower index.  A larger key
@@ -236,6 +273,14 @@ __device__ __forceinline__ uint32_t index_of(uint64_t key) { return 0xffffffffu 
 // scale * (x - m) - log(s): minus infinity for a masked place and for every place of a row that is masked throughout
 __device__ __forceinline__ float logprob_of(float x, float m, float total, float scale) {
   return x == neg_inf() && !isnan(m) && !isnan(total) ? neg_inf() : __fsub_rn(__fmul_rn(__fsub_rn(x, m), scale), total);
+}
+
+// Copies `bytes` (a multiple of 16, both ends on 16-byte boundaries) into shared memory; they count on `bar`.
+__device__ __forceinline__ void copy_in(void* to, const void* from, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   (uint32_t)__cvta_generic_to_shared(to)),
+               "l"(from), "r"(bytes), "r"((uint32_t)__cvta_generic_to_shared(bar))
+               : "memory");
 }
 
 // ---- a row shared by the blocks of a cluster --------------------------------------------------

@@ -468,18 +468,22 @@ struct GradArgs {
   float scale;
 };
 
-// What the gradient of a row is made of: dx = 2^d (at + bt d) with d = (x - m) scale log2(e), and the target's own share.
-// 1 / sum is taken once a row as e^-L and not within the exponent, where L ~ 10 would cost the last bits of every place.
+// What the gradient of a row is made of: dx = 2^d (at + bt d), and the target's own share.  d is x c2 - mc, or (x - base) c2
+// where the row's largest logit is not of an ordinary size (take in vocab.cuh has the same two forms).  1 / sum is taken
+// once a row as e^-L and not within the exponent, where L ~ 10 would cost the last bits of every place.
 struct GradRow {
-  float base, at, bt, own;
+  float minus, at, bt, own;  // minus: -mc, or -base
+  bool wide;
   uint32_t target;
 };
 
-__device__ __forceinline__ GradRow grad_row(const GradArgs& a, uint64_t r) {
+__device__ __forceinline__ GradRow grad_row(const GradArgs& a, uint64_t r, float c2) {
   GradRow w;
   const float* st = static_cast<const float*>(a.stats.data) + row_at(a.g, a.stats, r);
   const float m = st[0], total = st[a.stats.inner];
-  w.base = base_of(m);
+  w.wide = is_wide(m, c2);
+  w.minus = w.wide ? -base_of(m) : -(m * c2);
+  const float off = w.wide ? 0.0f : __fmaf_rn(m, c2, w.minus);  // m c2 - mc
   w.target = 0xffffffffu;
   float g = 0.0f, h = 0.0f, ent = 0.0f;
   if (a.d_logprob.data) {
@@ -493,10 +497,10 @@ __device__ __forceinline__ GradRow grad_row(const GradArgs& a, uint64_t r) {
     h = static_cast<const float*>(a.d_entropy.data)[row_at(a.g, a.d_entropy, r)];
     ent = static_cast<const float*>(a.entropy.data)[row_at(a.g, a.entropy, r)];
   }
-  const float per = a.scale * expf(-total);
+  const float per = a.scale * expf(-total) * ex2(-off);
   w.own = g * a.scale;
-  w.at = -per * (g + h * (ent - total));
   w.bt = -per * h * kLn2;
+  w.at = -per * (g + h * (ent - total - off * kLn2));
   if (m == neg_inf()) {  // masked throughout: there is no distribution, and no gradient
     w.at = w.bt = 0.0f;
     w.target = 0xffffffffu;
@@ -504,23 +508,112 @@ __device__ __forceinline__ GradRow grad_row(const GradArgs& a, uint64_t r) {
   return w;
 }
 
+// ENT: with the entropy's share.  Without it bt is 0 and a masked place needs no bound on d: 2^-inf at = 0.
+template <bool ENT>
 __device__ __forceinline__ float grad_of(float x, const GradRow& w, float c2) {
-  const float d = max_nan((x - w.base) * c2, kFar);
+  float d = w.wide ? (x + w.minus) * c2 : __fmaf_rn(x, c2, w.minus);
+  if constexpr (!ENT) return ex2(d) * w.at;
+  d = max_nan(d, kFar);
   return ex2(d) * __fmaf_rn(w.bt, d, w.at);
 }
 
-template <int DT>
-__global__ void __launch_bounds__(kThreads) token_logprobs_backward_strided(GradArgs a) {
+constexpr int kGradThreads = 256;
+
+template <int DT, bool ENT>
+__global__ void __launch_bounds__(kGradThreads) token_logprobs_backward_strided(GradArgs a) {
   using E = Elem<DT>;
   const float c2 = a.scale * kLog2e;
   for (uint64_t r = blockIdx.x; r < a.g.rows; r += gridDim.x) {
     const typename E::T* x = static_cast<const typename E::T*>(a.x.data) + row_at(a.g, a.x, r);
     typename E::T* dx = static_cast<typename E::T*>(a.dx.data) + row_at(a.g, a.dx, r);
-    const GradRow w = grad_row(a, r);
-    for (uint32_t j = threadIdx.x; j < a.vocab; j += kThreads) {
-      float v = grad_of(E::up(x[j * a.x.inner]), w, c2);
+    const GradRow w = grad_row(a, r, c2);
+    for (uint32_t j = threadIdx.x; j < a.vocab; j += kGradThreads) {
+      float v = grad_of<ENT>(E::up(x[j * a.x.inner]), w, c2);
       if (j == w.target) v += w.own;
       dx[j * a.dx.inner] = E::down(v);
+    }
+  }
+}
+
+// The vocabulary as the unit axis: a block has `steps` steps of kGradUnroll vectors a thread of one row, with all of a
+// step's loads on the way before the first is used.  The vectors are those of dx, so that every store is a whole one; where
+// x starts elsewhere within 16 bytes (an odd vocabulary against padded rows), a vector of it is two aligned loads, shifted.
+// The first and the last such vector, whose aligned loads would leave the row, and the places around the vectors are read
+// one by one.
+constexpr int kGradUnroll = 4;
+
+// MOVED: some row of x starts elsewhere within 16 bytes than the same row of dx.
+template <int DT, bool ENT, bool MOVED>
+__global__ void __launch_bounds__(kGradThreads, MOVED ? 4 : 6) token_logprobs_backward_rows(GradArgs a, uint32_t tiles, uint32_t steps) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  constexpr uint32_t kE = Vec<DT>::kElems;
+  const float c2 = a.scale * kLog2e;
+  const uint64_t items = a.g.rows * tiles;
+  for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const uint64_t r = item / tiles;
+    const uint32_t tile = (uint32_t)(item - r * tiles);
+    const T* x = static_cast<const T*>(a.x.data) + row_at(a.g, a.x, r);
+    T* dx = static_cast<T*>(a.dx.data) + row_at(a.g, a.dx, r);
+    const Span span = span_of<DT>(dx, a.vocab);
+    const char* xv = reinterpret_cast<const char*>(x + span.head);  // where vector 0 of dx reads
+    uint4* dv = reinterpret_cast<uint4*>(dx + span.head);
+    const uint32_t shift = reinterpret_cast<uintptr_t>(xv) & 15;
+    const uint32_t step = kGradUnroll * kGradThreads;
+    const uint32_t from = tile * steps * step, to = min(span.vecs, from + steps * step);
+    bool ready = false;
+    GradRow w;
+    for (uint32_t v0 = from; v0 < to; v0 += step) {
+      uint4 q[kGradUnroll];
+#pragma unroll
+      for (int u = 0; u < kGradUnroll; u++) {
+        const uint32_t v = v0 + u * kGradThreads + threadIdx.x;
+        if (v >= to) break;
+        const char* at = xv + (uint64_t)v * 16;
+        if (!MOVED || shift == 0) {
+          q[u] = *reinterpret_cast<const uint4*>(at);
+        } else if (at - shift >= reinterpret_cast<const char*>(x) && at - shift + 32 <= reinterpret_cast<const char*>(x + a.vocab)) {
+          const uint4* two = reinterpret_cast<const uint4*>(at - shift);
+          q[u] = shifted(__ldg(two), __ldg(two + 1), shift);
+        } else {
+          q[u] = one_by_one<DT>(at);
+        }
+      }
+      if (!ready) w = grad_row(a, r, c2);
+      ready = true;
+#pragma unroll
+      for (int u = 0; u < kGradUnroll; u++) {
+        const uint32_t v = v0 + u * kGradThreads + threadIdx.x;
+        if (v >= to) break;
+        float2 y[kE / 2];
+        const float2 minus = both(w.minus), c = both(c2), at = both(w.at), bt = both(w.bt);
+#pragma unroll
+        for (uint32_t i = 0; i < kE / 2; i++) {
+          const float2 p = Vec<DT>::pair(q[u], i);
+          float2 d = w.wide ? __fmul2_rn(__fadd2_rn(p, minus), c) : __ffma2_rn(p, c, minus);
+          if constexpr (ENT) d = make_float2(max_nan(d.x, kFar), max_nan(d.y, kFar));
+          y[i] = __fmul2_rn(make_float2(ex2(d.x), ex2(d.y)), ENT ? __ffma2_rn(bt, d, at) : at);
+        }
+        const uint32_t own = w.target - (span.head + v * kE);
+        if (own < kE) {
+#pragma unroll
+          for (uint32_t i = 0; i < kE / 2; i++) {
+            if (own == 2 * i) y[i].x += w.own;
+            if (own == 2 * i + 1) y[i].y += w.own;
+          }
+        }
+        dv[v] = Vec<DT>::pack(y);
+      }
+    }
+    if (tile == 0 && threadIdx.x < 16) {
+      const uint32_t i = threadIdx.x & 7;
+      if (threadIdx.x < 8 ? i < span.head : i < span.tail) {
+        const uint32_t j = threadIdx.x < 8 ? i : span.head + span.vecs * kE + i;
+        if (!ready) w = grad_row(a, r, c2);
+        float v = grad_of<ENT>(E::up(x[j]), w, c2);
+        if (j == w.target) v += w.own;
+        dx[j] = E::down(v);
+      }
     }
   }
 }
@@ -582,6 +675,30 @@ cudaError_t launch_rows(const lc_context* ctx, const ScoreArgs& a, cudaStream_t 
   cfg.attrs = at;
   cfg.numAttrs = s.cluster > 1 ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, a, s.cluster, s.per_slot);
+}
+
+template <int DT, bool ENT>
+void launch_backward(const lc_context* ctx, const GradArgs& a, bool unit, cudaStream_t stream) {
+  if (!unit) {
+    token_logprobs_backward_strided<DT, ENT><<<(unsigned)std::min<uint64_t>(a.g.rows, kMaxGrid), kGradThreads, 0, stream>>>(a);
+    return;
+  }
+  // blocks of up to 4 steps, fewer where that leaves the device idle
+  constexpr uint64_t kStep = (uint64_t)kGradUnroll * kGradThreads;
+  const uint64_t vecs = a.vocab / Vec<DT>::kElems, all = std::max<uint64_t>(1, (vecs + kStep - 1) / kStep);
+  uint32_t steps = 4;
+  while (steps > 1 && a.g.rows * ((all + steps - 1) / steps) < 12ull * ctx->sm_count) steps /= 2;
+  const uint32_t tiles = (uint32_t)((all + steps - 1) / steps);
+  const unsigned grid = (unsigned)std::min<uint64_t>(a.g.rows * tiles, 0x7fffffffull);
+  const bool moved = apart(a.g, a.x, a.dx, 16 / Vec<DT>::kElems);
+  auto kernel = moved ? token_logprobs_backward_rows<DT, ENT, true> : token_logprobs_backward_rows<DT, ENT, false>;
+  kernel<<<grid, kGradThreads, 0, stream>>>(a, tiles, steps);
+}
+
+template <int DT>
+void launch_backward(const lc_context* ctx, const GradArgs& a, bool unit, cudaStream_t stream) {
+  if (a.d_entropy.data) launch_backward<DT, true>(ctx, a, unit, stream);
+  else launch_backward<DT, false>(ctx, a, unit, stream);
 }
 
 unsigned row_grid(uint64_t rows) { return (unsigned)std::min<uint64_t>(rows, kMaxGrid); }
@@ -681,11 +798,11 @@ lc_status lc_encode_token_logprobs_backward(lc_context* ctx, void* stream, const
   a.scale = scale;
   DeviceGuard on(ctx->device);
   cudaStream_t s = stream_of(ctx, stream);
-  const unsigned grid = row_grid(a.g.rows);
-  if (logits->dtype == LC_F32) token_logprobs_backward_strided<LC_F32><<<grid, kThreads, 0, s>>>(a);
-  else if (logits->dtype == LC_F16) token_logprobs_backward_strided<LC_F16><<<grid, kThreads, 0, s>>>(a);
-  else token_logprobs_backward_strided<LC_BF16><<<grid, kThreads, 0, s>>>(a);
-  return launched(ctx, "token_logprobs_backward_strided");
+  const bool unit = a.vocab == 1 || (a.x.inner == 1 && a.dx.inner == 1);
+  if (logits->dtype == LC_F32) launch_backward<LC_F32>(ctx, a, unit, s);
+  else if (logits->dtype == LC_F16) launch_backward<LC_F16>(ctx, a, unit, s);
+  else launch_backward<LC_BF16>(ctx, a, unit, s);
+  return launched(ctx, unit ? "token_logprobs_backward_rows" : "token_logprobs_backward_strided");
 }
 
 }  // extern "C"

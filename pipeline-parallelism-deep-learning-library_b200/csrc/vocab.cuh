@@ -132,6 +132,31 @@ __device__ __forceinline__ uint4 load_once(const void* p) {
   return q;
 }
 
+// 16 bytes that start `shift` bytes (0 to 15, a multiple of the element's size) into the 32 of lo and hi.
+__device__ __forceinline__ uint4 shifted(const uint4& lo, const uint4& hi, uint32_t shift) {
+  const uint32_t bits = (shift & 3) * 8;
+  uint32_t a, b, c, d, e;
+  switch (shift >> 2) {  // the same for a whole row
+    case 0: a = lo.x; b = lo.y; c = lo.z; d = lo.w; e = hi.x; break;
+    case 1: a = lo.y; b = lo.z; c = lo.w; d = hi.x; e = hi.y; break;
+    case 2: a = lo.z; b = lo.w; c = hi.x; d = hi.y; e = hi.z; break;
+    default: a = lo.w; b = hi.x; c = hi.y; d = hi.z; e = hi.w;
+  }
+  return make_uint4(__funnelshift_r(a, b, bits), __funnelshift_r(b, c, bits), __funnelshift_r(c, d, bits), __funnelshift_r(d, e, bits));
+}
+
+// 16 bytes that start anywhere, place by place.
+template <int DT>
+__device__ __forceinline__ uint4 one_by_one(const void* at) {
+  if constexpr (DT == LC_F32) {
+    const uint32_t* p = static_cast<const uint32_t*>(at);
+    return make_uint4(p[0], p[1], p[2], p[3]);
+  } else {
+    const uint16_t* p = static_cast<const uint16_t*>(at);
+    return make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16, p[6] | (uint32_t)p[7] << 16);
+  }
+}
+
 struct Soft {
   float m, s, t;
 };

@@ -30,6 +30,14 @@ struct RowOperand {
   uint64_t st[LC_MAX_RANK];
 };
 
+// Whether some row of `a` starts elsewhere within 16 bytes than the same row of `b`, `size` bytes an element.
+inline bool apart(const Rows& g, const RowOperand& a, const RowOperand& b, uint64_t size) {
+  uint64_t off = (reinterpret_cast<uintptr_t>(a.data) + a.offset * size) ^ (reinterpret_cast<uintptr_t>(b.data) + b.offset * size);
+  for (int d = 0; d < g.rank; d++)
+    if (g.shape[d] > 1) off |= (a.st[d] - b.st[d]) * size;
+  return off % 16 != 0;
+}
+
 // Makes the context's device the current one while a call lasts: a caller may be on another device.
 class DeviceGuard {
  public:

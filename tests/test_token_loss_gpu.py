@@ -300,6 +300,11 @@ def check_scores_grad(ctx, x, t, scale, g, h, what="", in_place=False):
     want = ref.s * (torch.where(dead, 0.0, gg) * (hot - p) - hh * p * (lp + ent))
     big = p * (gg.abs() + hh.abs() * (lp.abs() + ent.abs() + total.nan_to_num(0, 0, 0).abs() + ref.absd))
     tol = ref.s * U * big * (3 * ref.absd + 24) + 4 * U * ref.s * gg.abs() * hot
+    # d = x c2 - mc with mc = m c2 (c2 = s log2 e) as it rounds, so d at the largest logit is off = m c2 - mc and not 0,
+    # |off| <= U |m c2|.  The row's constant takes bt off away again (|bt| <= s |h| p there), as it rounds: off by U |bt off|,
+    # and by as much again in its own sum.  So even where everything else is 0 there may be 2 U |bt off| <= 2 U^2 s |h| |m c2|.
+    m = torch.where(ref.m.isfinite(), ref.m, 0.0).abs()[:, None]
+    tol = tol + 2 * U * U * ref.s * hh.abs() * p * m * (ref.s * 1.4427)
     tol = tol + want.abs() * (torch.finfo(x.dtype).eps / 2) + tiny(x.dtype)
     close(dx, want, tol, what + " dlogits")
     return dx

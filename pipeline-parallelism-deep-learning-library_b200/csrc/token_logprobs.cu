@@ -535,20 +535,54 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_backward_strided(
   }
 }
 
+// 16 bytes of dx from 16 bytes of x whose first place is j.
+template <int DT, bool ENT>
+__device__ __forceinline__ uint4 grad_vec(const uint4& q, uint32_t j, const GradRow& w, float c2) {
+  constexpr uint32_t kE = Vec<DT>::kElems;
+  float2 y[kE / 2];
+  const float2 minus = both(w.minus), c = both(c2), at = both(w.at), bt = both(w.bt);
+  if (!w.wide) {
+#pragma unroll
+    for (uint32_t i = 0; i < kE / 2; i++) y[i] = __ffma2_rn(Vec<DT>::pair(q, i), c, minus);
+  } else {
+#pragma unroll
+    for (uint32_t i = 0; i < kE / 2; i++) y[i] = __fmul2_rn(__fadd2_rn(Vec<DT>::pair(q, i), minus), c);
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < kE / 2; i++) {
+    float2 d = y[i];
+    if constexpr (ENT) d = make_float2(max_nan(d.x, kFar), max_nan(d.y, kFar));
+    y[i] = __fmul2_rn(make_float2(ex2(d.x), ex2(d.y)), ENT ? __ffma2_rn(bt, d, at) : at);
+  }
+  const uint32_t own = w.target - j;
+  if (own < kE) {
+#pragma unroll
+    for (uint32_t i = 0; i < kE / 2; i++) {
+      if (own == 2 * i) y[i].x += w.own;
+      if (own == 2 * i + 1) y[i].y += w.own;
+    }
+  }
+  return Vec<DT>::pack(y);
+}
+
 // The vocabulary as the unit axis: a block has `steps` steps of kGradUnroll vectors a thread of one row, with all of a
-// step's loads on the way before the first is used.  The vectors are those of dx, so that every store is a whole one; where
-// x starts elsewhere within 16 bytes (an odd vocabulary against padded rows), a vector of it is two aligned loads, shifted.
-// The first and the last such vector, whose aligned loads would leave the row, and the places around the vectors are read
-// one by one.
+// step's loads on the way before the first is used.  The vectors are those of
+// dx, so that every store is a whole one.  MOVED: some row of x starts elsewhere within 16 bytes (an odd vocabulary against
+// padded rows).  A vector of it then is cut out of two aligned ones, of which the second comes from the next lane (a
+// warp's vectors of a step follow one another), or at the end of a warp's vectors from a load of its own.  In steps that reach the row's ends the vectors are read one by one, as
+// are the places around them.
 constexpr int kGradUnroll = 4;
 
-// MOVED: some row of x starts elsewhere within 16 bytes than the same row of dx.
 template <int DT, bool ENT, bool MOVED>
-__global__ void __launch_bounds__(kGradThreads, MOVED ? 4 : 6) token_logprobs_backward_rows(GradArgs a, uint32_t tiles, uint32_t steps) {
+__global__ void __launch_bounds__(kGradThreads, 4) token_logprobs_backward_rows(GradArgs a, uint32_t tiles, uint32_t steps) {
   using E = Elem<DT>;
   using T = typename E::T;
   constexpr uint32_t kE = Vec<DT>::kElems;
+  constexpr int kU = kGradUnroll;
   const float c2 = a.scale * kLog2e;
+  const uint32_t lane = threadIdx.x & 31;
+  // vectors of a thread: where the first of a step lies, and how far apart they are
+  const uint32_t place = MOVED ? (threadIdx.x & ~31u) * kU + lane : threadIdx.x, apart = MOVED ? 32 : blockDim.x;
   const uint64_t items = a.g.rows * tiles;
   for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const uint64_t r = item / tiles;
@@ -558,52 +592,46 @@ __global__ void __launch_bounds__(kGradThreads, MOVED ? 4 : 6) token_logprobs_ba
     const Span span = span_of<DT>(dx, a.vocab);
     const char* xv = reinterpret_cast<const char*>(x + span.head);  // where vector 0 of dx reads
     uint4* dv = reinterpret_cast<uint4*>(dx + span.head);
-    const uint32_t shift = reinterpret_cast<uintptr_t>(xv) & 15;
-    const uint32_t step = kGradUnroll * kGradThreads;
-    const uint32_t from = tile * steps * step, to = min(span.vecs, from + steps * step);
+    const uint32_t shift = MOVED ? reinterpret_cast<uintptr_t>(xv) & 15 : 0;
+    // the aligned vectors of x that begin and end within the row, where vector v is cut out of v and v + 1
+    const uint32_t first = MOVED && xv - shift < reinterpret_cast<const char*>(x) ? 1 : 0;
+    const uint32_t count = MOVED ? (uint32_t)((reinterpret_cast<const char*>(x + a.vocab) - (xv - shift)) / 16) : 0;
+    const uint32_t step = kU * blockDim.x;
+    const uint32_t from = min(span.vecs, tile * steps * step), to = min(span.vecs, from + steps * step);
     bool ready = false;
     GradRow w;
     for (uint32_t v0 = from; v0 < to; v0 += step) {
-      uint4 q[kGradUnroll];
+      uint4 q[kU];
+      const uint32_t v = v0 + place;
+      if (!MOVED || shift == 0) {
 #pragma unroll
-      for (int u = 0; u < kGradUnroll; u++) {
-        const uint32_t v = v0 + u * kGradThreads + threadIdx.x;
-        if (v >= to) break;
-        const char* at = xv + (uint64_t)v * 16;
-        if (!MOVED || shift == 0) {
-          q[u] = *reinterpret_cast<const uint4*>(at);
-        } else if (at - shift >= reinterpret_cast<const char*>(x) && at - shift + 32 <= reinterpret_cast<const char*>(x + a.vocab)) {
-          const uint4* two = reinterpret_cast<const uint4*>(at - shift);
-          q[u] = shifted(__ldg(two), __ldg(two + 1), shift);
-        } else {
-          q[u] = one_by_one<DT>(at);
+        for (int u = 0; u < kU; u++)
+          if (v + u * apart < to) q[u] = *reinterpret_cast<const uint4*>(xv + (uint64_t)(v + u * apart) * 16);
+      } else if (v0 >= first && v0 + step < count && v0 + step <= to) {
+        const uint4* xa = reinterpret_cast<const uint4*>(xv - shift) + v;
+#pragma unroll
+        for (int u = 0; u < kU; u++) q[u] = __ldg(xa + u * apart);
+        uint4 last;
+        if (lane == 31) last = __ldg(xa + kU * apart - 31);
+#pragma unroll
+        for (int u = 0; u < kU; u++) {
+          uint4 give = q[u];
+          if (u + 1 < kU && lane == 0) give = q[u + 1 < kU ? u + 1 : u];
+          uint4 next = make_uint4(__shfl_sync(0xffffffffu, give.x, lane + 1), __shfl_sync(0xffffffffu, give.y, lane + 1),
+                                  __shfl_sync(0xffffffffu, give.z, lane + 1), __shfl_sync(0xffffffffu, give.w, lane + 1));
+          if (u + 1 == kU && lane == 31) next = last;
+          q[u] = shifted(q[u], next, shift);
         }
+      } else {
+#pragma unroll
+        for (int u = 0; u < kU; u++)
+          if (v + u * apart < to) q[u] = one_by_one<DT>(xv + (uint64_t)(v + u * apart) * 16);
       }
       if (!ready) w = grad_row(a, r, c2);
       ready = true;
 #pragma unroll
-      for (int u = 0; u < kGradUnroll; u++) {
-        const uint32_t v = v0 + u * kGradThreads + threadIdx.x;
-        if (v >= to) break;
-        float2 y[kE / 2];
-        const float2 minus = both(w.minus), c = both(c2), at = both(w.at), bt = both(w.bt);
-#pragma unroll
-        for (uint32_t i = 0; i < kE / 2; i++) {
-          const float2 p = Vec<DT>::pair(q[u], i);
-          float2 d = w.wide ? __fmul2_rn(__fadd2_rn(p, minus), c) : __ffma2_rn(p, c, minus);
-          if constexpr (ENT) d = make_float2(max_nan(d.x, kFar), max_nan(d.y, kFar));
-          y[i] = __fmul2_rn(make_float2(ex2(d.x), ex2(d.y)), ENT ? __ffma2_rn(bt, d, at) : at);
-        }
-        const uint32_t own = w.target - (span.head + v * kE);
-        if (own < kE) {
-#pragma unroll
-          for (uint32_t i = 0; i < kE / 2; i++) {
-            if (own == 2 * i) y[i].x += w.own;
-            if (own == 2 * i + 1) y[i].y += w.own;
-          }
-        }
-        dv[v] = Vec<DT>::pack(y);
-      }
+      for (int u = 0; u < kU; u++)
+        if (v + u * apart < to) __stcs(dv + v + u * apart, grad_vec<DT, ENT>(q[u], span.head + (v + u * apart) * kE, w, c2));
     }
     if (tile == 0 && threadIdx.x < 16) {
       const uint32_t i = threadIdx.x & 7;
@@ -683,16 +711,17 @@ void launch_backward(const lc_context* ctx, const GradArgs& a, bool unit, cudaSt
     token_logprobs_backward_strided<DT, ENT><<<(unsigned)std::min<uint64_t>(a.g.rows, kMaxGrid), kGradThreads, 0, stream>>>(a);
     return;
   }
-  // blocks of up to 4 steps, fewer where that leaves the device idle
-  constexpr uint64_t kStep = (uint64_t)kGradUnroll * kGradThreads;
-  const uint64_t vecs = a.vocab / Vec<DT>::kElems, all = std::max<uint64_t>(1, (vecs + kStep - 1) / kStep);
+  // short rows take a small block; long ones blocks of up to 4 steps, fewer where that leaves the device idle
+  const uint64_t vecs = a.vocab / Vec<DT>::kElems, busy = (vecs + kGradUnroll - 1) / kGradUnroll;
+  const uint32_t threads = (uint32_t)std::min<uint64_t>(kGradThreads, std::max<uint64_t>(32, (busy + 31) / 32 * 32));
+  const uint64_t step = (uint64_t)kGradUnroll * threads, all = std::max<uint64_t>(1, (vecs + step - 1) / step);
   uint32_t steps = 4;
   while (steps > 1 && a.g.rows * ((all + steps - 1) / steps) < 12ull * ctx->sm_count) steps /= 2;
   const uint32_t tiles = (uint32_t)((all + steps - 1) / steps);
   const unsigned grid = (unsigned)std::min<uint64_t>(a.g.rows * tiles, 0x7fffffffull);
   const bool moved = apart(a.g, a.x, a.dx, 16 / Vec<DT>::kElems);
   auto kernel = moved ? token_logprobs_backward_rows<DT, ENT, true> : token_logprobs_backward_rows<DT, ENT, false>;
-  kernel<<<grid, kGradThreads, 0, stream>>>(a, tiles, steps);
+  kernel<<<grid, threads, 0, stream>>>(a, tiles, steps);
 }
 
 template <int DT>

@@ -134,15 +134,11 @@ __device__ __forceinline__ uint4 load_once(const void* p) {
 
 // 16 bytes that start `shift` bytes (0 to 15, a multiple of the element's size) into the 32 of lo and hi.
 __device__ __forceinline__ uint4 shifted(const uint4& lo, const uint4& hi, uint32_t shift) {
-  const uint32_t bits = (shift & 3) * 8;
-  uint32_t a, b, c, d, e;
-  switch (shift >> 2) {  // the same for a whole row
-    case 0: a = lo.x; b = lo.y; c = lo.z; d = lo.w; e = hi.x; break;
-    case 1: a = lo.y; b = lo.z; c = lo.w; d = hi.x; e = hi.y; break;
-    case 2: a = lo.z; b = lo.w; c = hi.x; d = hi.y; e = hi.z; break;
-    default: a = lo.w; b = hi.x; c = hi.y; d = hi.z; e = hi.w;
-  }
-  return make_uint4(__funnelshift_r(a, b, bits), __funnelshift_r(b, c, bits), __funnelshift_r(c, d, bits), __funnelshift_r(d, e, bits));
+  const bool two = shift & 8, one = shift & 4;
+  const uint32_t a = two ? lo.z : lo.x, b = two ? lo.w : lo.y, c = two ? hi.x : lo.z, d = two ? hi.y : lo.w, e = two ? hi.z : hi.x,
+                 f = two ? hi.w : hi.y;
+  const uint32_t g = one ? b : a, h = one ? c : b, i = one ? d : c, j = one ? e : d, k = one ? f : e, bits = (shift & 3) * 8;
+  return make_uint4(__funnelshift_r(g, h, bits), __funnelshift_r(h, i, bits), __funnelshift_r(i, j, bits), __funnelshift_r(j, k, bits));
 }
 
 // 16 bytes that start anywhere, place by place.

@@ -14,6 +14,7 @@
 // form is e^(scale (x_j - mt)) (c e^(scale (mt - m)) / S - r / St), which stands also where Q underflows.
 #include <cmath>
 
+#include "ptx.cuh"
 #include "vocab.cuh"
 
 namespace {
@@ -203,6 +204,306 @@ __global__ void __launch_bounds__(kThreads) distill_strided(DistillArgs a) {
   }
 }
 
+// ---- the vocabulary as the unit axis -----------------------------------------------------------
+//
+// A cluster of blocks a row, each with a slice of it in shared memory: the copy engine brings the slice in while the block
+// works out the teacher's list, the list's places in it are set to minus infinity, and the sums and the gradient are two
+// passes over shared memory.  So a row crosses HBM once each way.  Between the passes the blocks tell one another their sums.
+// A slice that does not fit comes in chunks, once for each pass.
+constexpr int kRowThreads = 256;
+constexpr int kUnroll = 4;
+constexpr uint32_t kMaxCluster = 8;
+
+// What a block tells the others of its cluster.
+struct Part {
+  float rest_m, rest_s, named_m, named_s;
+  double p, dot;  // sum P and sum P scale (x - named_m) over the list's places in the slice
+};
+
+// A thread's entry of the list.
+struct Entry {
+  uint32_t id;  // ~0 if it does not stand
+  double p;     // 64 bits: the loss has sum P scale x beside sum P log P, which cancel to a small part
+};
+
+__device__ __forceinline__ double2 block_sum(double2 v, double2* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+  }
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x / 32] = v;
+  __syncthreads();
+  v = red[0];
+  for (int w = 1; w < (int)blockDim.x / 32; w++) v = make_double2(v.x + red[w].x, v.y + red[w].y);
+  __syncthreads();
+  return v;
+}
+
+// The teacher's list of row r, an entry a thread; `sums`: sum P and sum P log P.
+__device__ __forceinline__ Entry read_entry(const DistillArgs& a, uint64_t r, uint32_t* ids, float* redf, double2* redd, double2* sums) {
+  const uint32_t k = threadIdx.x;
+  const bool here = k < a.list;
+  Entry e{0xffffffffu, 0.0};
+  float z = neg_inf();
+  if (here) {
+    e.id = static_cast<const uint32_t*>(a.ids.data)[row_at(a.g, a.ids, r) + k * a.ids.inner];
+    z = teacher_value(a, row_at(a.g, a.teacher, r) + k * a.teacher.inner);
+    ids[k] = e.id;
+  }
+  __syncthreads();
+  bool stands = here && e.id < a.vocab;
+  if (stands)
+    for (uint32_t i = 0; i < k; i++) stands = stands && ids[i] != e.id;
+  if (!stands) {
+    e.id = 0xffffffffu;
+    z = neg_inf();
+  }
+  double lz = z, w = 0.0;
+  if (!a.tail) {
+    const float top = base_of(block_max(z, redf));
+    lz = (double)a.scale * ((double)z - (double)top);
+  }
+  if (stands) w = exp(lz);
+  // of the renormalised P = w / total: sum P log P = (sum w lz) / total - log total
+  const double2 t = block_sum(make_double2(w, w > 0.0 || isnan(w) ? w * lz : 0.0), redd);
+  if (a.tail) {
+    *sums = t;
+    e.p = w;
+  } else if (t.x > 0.0 || isnan(t.x)) {
+    *sums = make_double2(isnan(t.x) ? t.x : 1.0, t.y / t.x - log(t.x));
+    e.p = w / t.x;
+  } else {  // no entry says anything
+    *sums = make_double2(0.0, 0.0);
+  }
+  return e;
+}
+
+// dx = coef 2^d outside the list, in the same two forms of d as take (vocab.cuh)
+struct Tail {
+  float minus, coef;
+  bool wide;
+};
+
+template <int DT>
+__device__ __forceinline__ uint4 tail_vec(const uint4& q, const Tail& w, float c2) {
+  constexpr int kP = Vec<DT>::kElems / 2;
+  float2 y[kP];
+  const float2 minus = both(w.minus), c = both(c2), coef = both(w.coef);
+  if (!w.wide) {
+#pragma unroll
+    for (int i = 0; i < kP; i++) y[i] = __ffma2_rn(Vec<DT>::pair(q, i), c, minus);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kP; i++) y[i] = __fmul2_rn(__fadd2_rn(Vec<DT>::pair(q, i), minus), c);
+  }
+#pragma unroll
+  for (int i = 0; i < kP; i++) y[i] = __fmul2_rn(make_float2(ex2(y[i].x), ex2(y[i].y)), coef);
+  return Vec<DT>::pack(y);
+}
+
+__device__ __forceinline__ float tail_of(float x, const Tail& w, float c2) {
+  return ex2(w.wide ? (x + w.minus) * c2 : __fmaf_rn(x, c2, w.minus)) * w.coef;
+}
+
+// chunk: vectors of shared memory; chunks: how many a slice takes.
+template <int DT, bool GRAD, bool MOVED>
+__global__ void __launch_bounds__(kRowThreads, 5) distill_rows(DistillArgs a, uint32_t cluster, uint32_t share, uint32_t chunk, int* err) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  constexpr uint32_t kE = Vec<DT>::kElems;
+  extern __shared__ __align__(128) uint4 data[];  // [chunk], and 16 bytes more
+  __shared__ uint64_t full;
+  __shared__ uint32_t ids[kMaxList];
+  __shared__ Soft red[2][kRowThreads / 32];
+  __shared__ float redf[kRowThreads / 32], edges[16];
+  __shared__ double2 redd[kRowThreads / 32];
+  __shared__ Part parts[kMaxCluster];
+  T* const in = reinterpret_cast<T*>(data);
+  const uint32_t rank = cluster > 1 ? cluster_rank() : 0;
+  const float c2 = a.scale * kLog2e;
+  if (threadIdx.x == 0) {
+    lcd::mbar_init(&full, 1);
+    lcd::fence_mbar_init();
+  }
+  __syncthreads();
+  uint32_t parity = 0;
+  // Cluster barriers alternate: every block's `parts` are free (at first: it has started), and they are filled.
+  if (cluster > 1) cluster_arrive();
+  for (uint64_t r = blockIdx.x / cluster; r < a.g.rows; r += gridDim.x / cluster) {
+    const T* x = static_cast<const T*>(a.x.data) + row_at(a.g, a.x, r);
+    const Span span = span_of<DT>(x, a.vocab);
+    const uint32_t from = min(span.vecs, rank * share), to = min(span.vecs, from + share);
+    const uint4* vec = reinterpret_cast<const uint4*>(x + span.head);
+    auto fetch = [&](uint32_t v0) {  // vectors v0 .. of the slice; the last reads of shared memory are behind a barrier
+      if (threadIdx.x == 0) {
+        lcd::fence_proxy_async_smem();
+        const uint32_t n = min(chunk, to - v0);
+        lcd::mbar_arrive_expect_tx(&full, n * 16);
+        copy_in(data, vec + v0, n * 16, &full);
+      }
+    };
+    if (from < to) fetch(from);
+    // the places before the vectors (0-7) and behind them (8-15) are block 0's
+    uint32_t edge_at = 0xffffffffu;
+    if (rank == 0 && threadIdx.x < 16) {
+      const uint32_t i = threadIdx.x & 7;
+      if (threadIdx.x < 8 ? i < span.head : i < span.tail) {
+        edge_at = threadIdx.x < 8 ? i : span.head + span.vecs * kE + i;
+        edges[threadIdx.x] = E::up(x[edge_at]);
+      }
+    }
+    const float d_loss = GRAD && a.d_loss.data ? static_cast<const float*>(a.d_loss.data)[row_at(a.g, a.d_loss, r)] : 1.0f;
+    double2 sums;
+    const Entry entry = read_entry(a, r, ids, redf, redd, &sums);
+    // where the entry's place lies: in the vectors (counted in places from the first of them), or among the edges
+    const uint32_t at = entry.id - span.head;
+    const bool in_vecs = entry.id != 0xffffffffu && entry.id >= span.head && at < span.vecs * kE;
+    float xk = neg_inf();
+    bool mine = false;
+    if (rank == 0 && entry.id != 0xffffffffu && !in_vecs) {
+      float* e = &edges[entry.id < span.head ? entry.id : 8 + at - span.vecs * kE];
+      xk = *e;
+      *e = neg_inf();
+      mine = true;
+    }
+    // takes the list's places out of the chunk that begins with vector v0
+    auto mark = [&](uint32_t v0, uint32_t n) {
+      if (in_vecs && at >= v0 * kE && at < (v0 + n) * kE) {
+        xk = E::up(in[at - v0 * kE]);
+        in[at - v0 * kE] = E::down(neg_inf());
+        mine = true;
+      }
+    };
+    Run run = empty_run();
+    for (uint32_t v0 = from; v0 < to; v0 += chunk) {
+      if (v0 > from) {
+        __syncthreads();
+        fetch(v0);
+      }
+      const uint32_t n = min(chunk, to - v0);
+      lcd::mbar_wait(&full, parity, err);
+      parity ^= 1;
+      mark(v0, n);
+      __syncthreads();
+      uint32_t i = threadIdx.x;
+      for (; i + (kUnroll - 1) * blockDim.x < n; i += kUnroll * blockDim.x) {
+        uint4 q[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; u++) q[u] = data[i + u * blockDim.x];
+        float top = Vec<DT>::top(q[0]);
+#pragma unroll
+        for (int u = 1; u < kUnroll; u++) top = max_nan(top, Vec<DT>::top(q[u]));
+        take<DT, kUnroll, false>(run, q, top, c2);
+      }
+      for (; i < n; i += blockDim.x) {
+        const uint4 q[1] = {data[i]};
+        take<DT, 1, false>(run, q, Vec<DT>::top(q[0]), c2);
+      }
+    }
+    if (from == to) __syncthreads();  // the edges are written and marked
+    Soft rest = soft_of(run, c2);
+    if (edge_at != 0xffffffffu) {
+      const float e = edges[threadIdx.x];
+      rest = merge(rest, Soft{e, e == neg_inf() ? 0.0f : 1.0f, 0.0f}, c2);
+    }
+    rest = block_merge(rest, c2, red[0]);
+    Soft named = block_merge(Soft{xk, xk == neg_inf() ? 0.0f : 1.0f, 0.0f}, c2, red[1]);
+    // P > 0 at a masked place makes the loss infinite; P = 0 there says nothing
+    const bool says = mine && entry.p != 0.0;
+    const double2 dots = block_sum(
+        says ? make_double2(entry.p, entry.p * ((double)a.scale * ((double)xk - (double)base_of(named.m)))) : make_double2(0.0, 0.0), redd);
+    if (cluster > 1) {
+      cluster_wait();
+      if (threadIdx.x < cluster) {
+        const uint32_t to_part = remote(&parts[rank], threadIdx.x);
+        store_remote(to_part, (uint64_t)__float_as_uint(rest.m) | (uint64_t)__float_as_uint(rest.s) << 32);
+        store_remote(to_part + 8, (uint64_t)__float_as_uint(named.m) | (uint64_t)__float_as_uint(named.s) << 32);
+        store_remote(to_part + 16, (uint64_t)__double_as_longlong(dots.x));
+        store_remote(to_part + 24, (uint64_t)__double_as_longlong(dots.y));
+      }
+      cluster_arrive();
+      cluster_wait();
+      rest = named = Soft{neg_inf(), 0.0f, 0.0f};
+      for (uint32_t c = 0; c < cluster; c++) {
+        rest = merge(rest, Soft{parts[c].rest_m, parts[c].rest_s, 0.0f}, c2);
+        named = merge(named, Soft{parts[c].named_m, parts[c].named_s, 0.0f}, c2);
+      }
+    }
+    const Soft all = merge(rest, named, c2);
+    // sum P scale (x - m) over the whole list
+    auto from_top = [&](double p, double d, float m) { return d + p * ((double)a.scale * ((double)base_of(m) - (double)base_of(all.m))); };
+    double dot;
+    if (cluster > 1) {
+      dot = 0.0;
+      for (uint32_t c = 0; c < cluster; c++) dot += from_top(parts[c].p, parts[c].dot, parts[c].named_m);
+      cluster_arrive();
+    } else {
+      dot = from_top(dots.x, dots.y, named.m);
+    }
+    double left = a.tail ? 1.0 - sums.x : 0.0;
+    if (left < 0.0 || rest.s == 0.0f) left = 0.0;
+    const float total = (float)(sums.x + left), tail = (float)left;
+    const float lead = (base_of(rest.m) - base_of(all.m)) * a.scale;  // at most 0 where it counts
+    if (a.loss.data && rank == 0 && threadIdx.x == 0) {
+      // sum P (log P - log q) with log q = scale (x - m) - log S
+      double loss = sums.y - (dot - sums.x * (double)logf(all.s));
+      if (all.s == 0.0f) loss = sums.x > 0.0 ? (double)__int_as_float(0x7f800000) : 0.0;
+      if (tail > 0.0f) loss += (double)(tail * (logf(tail) - (logf(rest.s) + lead - logf(all.s))));
+      static_cast<float*>(a.loss.data)[row_at(a.g, a.loss, r)] = (float)loss;
+    }
+    if constexpr (GRAD) {
+      float weight = d_loss * a.scale;
+      // against mc / c2, which is where 2^d is taken from (vocab.cuh)
+      Tail w;
+      w.wide = is_wide(rest.m, c2);
+      w.minus = w.wide ? -base_of(rest.m) : -(rest.m * c2);
+      const float off = w.wide ? 0.0f : __fmaf_rn(rest.m, c2, w.minus);
+      w.coef = rest.s == 0.0f ? 0.0f : (total * expf(lead) / all.s - tail / rest.s) * weight * ex2(-off);
+      const float in_coef = all.s == 0.0f ? 0.0f : total / all.s * weight;
+      if (all.m == neg_inf()) weight = 0.0f;  // masked throughout: there is no distribution, and no gradient
+      T* dx = static_cast<T*>(a.dx.data) + row_at(a.g, a.dx, r);
+      for (uint32_t v0 = from; v0 < to; v0 += chunk) {
+        const uint32_t n = min(chunk, to - v0);
+        if (to - from > chunk) {  // the slice's other chunks have been here since
+          __syncthreads();
+          fetch(v0);
+          lcd::mbar_wait(&full, parity, err);
+          parity ^= 1;
+          mark(v0, n);
+          __syncthreads();
+        }
+        T* const out = dx + span.head + (uint64_t)v0 * kE;
+        if constexpr (!MOVED) {
+          uint4* const ov = reinterpret_cast<uint4*>(out);
+#pragma unroll 4
+          for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) __stcs(ov + i, tail_vec<DT>(data[i], w, c2));
+        } else {
+          // whole vectors of dx, cut out of shared memory; the places around them one by one
+          const Span os = span_of<DT>(out, n * kE);
+          uint4* const ov = reinterpret_cast<uint4*>(out + os.head);
+          const uint32_t shift = os.head * (16 / kE);
+#pragma unroll 4
+          for (uint32_t i = threadIdx.x; i < os.vecs; i += blockDim.x)
+            __stcs(ov + i, tail_vec<DT>(shifted(data[i], data[i + 1], shift), w, c2));
+          if (threadIdx.x < 16) {
+            const uint32_t i = threadIdx.x & 7;
+            if (threadIdx.x < 8 ? i < os.head : i < os.tail) {
+              const uint32_t j = threadIdx.x < 8 ? i : os.head + os.vecs * kE + i;
+              out[j] = E::down(tail_of(E::up(in[j]), w, c2));
+            }
+          }
+        }
+      }
+      if (edge_at != 0xffffffffu) dx[edge_at] = E::down(tail_of(edges[threadIdx.x], w, c2));
+      __syncthreads();
+      if (mine) dx[entry.id] = E::down(ex2((xk - base_of(all.m)) * c2) * in_coef - weight * (float)entry.p);
+    }
+    __syncthreads();
+  }
+  if (cluster > 1) cluster_wait();
+}
+
 lc_status launched(lc_context* ctx, const char* name) {
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return lc::cuda_fail(e, name);
@@ -210,11 +511,51 @@ lc_status launched(lc_context* ctx, const char* name) {
   return LC_OK;
 }
 
+// Slices of 32 KB, so that several blocks share an SM and one computes while another waits for its slice or stores; smaller
+// ones where there are few rows.  Up to 96 KB of a slice is held at once.
+constexpr uint64_t kSlice = 32 << 10, kSmallSlice = 8 << 10, kHeld = 96 << 10;
+
+template <int DT, bool GRAD>
+cudaError_t launch_rows(const lc_context* ctx, const DistillArgs& a, cudaStream_t stream) {
+  constexpr uint64_t kE = Vec<DT>::kElems;
+  const uint64_t vecs = a.vocab / kE;
+  uint32_t cluster = 1;
+  while (cluster < kMaxCluster && (vecs * 16 > kSlice * cluster ||
+                                   (a.g.rows * cluster < 2ull * ctx->sm_count && vecs * 16 > kSmallSlice * cluster)))
+    cluster *= 2;
+  const uint64_t share = std::max<uint64_t>(1, (vecs + cluster - 1) / cluster), chunk = std::min<uint64_t>(share, kHeld / 16);
+  const uint64_t busy = std::max<uint64_t>((chunk + kUnroll - 1) / kUnroll, a.list);
+  const uint32_t threads = (uint32_t)std::min<uint64_t>(kRowThreads, std::max<uint64_t>(32, (busy + 31) / 32 * 32));
+  const bool moved = GRAD && apart(a.g, a.x, a.dx, 16 / kE);
+  void (*kernel)(DistillArgs, uint32_t, uint32_t, uint32_t, int*) = moved ? distill_rows<DT, GRAD, GRAD> : distill_rows<DT, GRAD, false>;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(std::min<uint64_t>(a.g.rows, kMaxGrid) * cluster));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = (chunk + 1) * 16;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes);
+  if (e != cudaSuccess) return e;
+  return cudaLaunchKernelEx(&cfg, kernel, a, cluster, (uint32_t)share, (uint32_t)chunk, ctx->d_error);
+}
+
+template <int DT, bool GRAD>
+cudaError_t launch(const lc_context* ctx, const DistillArgs& a, bool unit, cudaStream_t stream) {
+  if (unit) return launch_rows<DT, GRAD>(ctx, a, stream);
+  distill_strided<DT, GRAD><<<(unsigned)std::min<uint64_t>(a.g.rows, kMaxGrid), kThreads, 0, stream>>>(a);
+  return cudaSuccess;
+}
+
 template <bool GRAD>
-void launch(const DistillArgs& a, int32_t dtype, unsigned grid, cudaStream_t s) {
-  if (dtype == LC_F32) distill_strided<LC_F32, GRAD><<<grid, kThreads, 0, s>>>(a);
-  else if (dtype == LC_F16) distill_strided<LC_F16, GRAD><<<grid, kThreads, 0, s>>>(a);
-  else distill_strided<LC_BF16, GRAD><<<grid, kThreads, 0, s>>>(a);
+cudaError_t launch(const lc_context* ctx, const DistillArgs& a, int32_t dtype, bool unit, cudaStream_t s) {
+  if (dtype == LC_F32) return launch<LC_F32, GRAD>(ctx, a, unit, s);
+  if (dtype == LC_F16) return launch<LC_F16, GRAD>(ctx, a, unit, s);
+  return launch<LC_BF16, GRAD>(ctx, a, unit, s);
 }
 
 lc_status distill(const char* op, lc_context* ctx, void* stream, const lc_view* logits, const lc_view* ids,
@@ -257,10 +598,11 @@ lc_status distill(const char* op, lc_context* ctx, void* stream, const lc_view* 
   a.scale = scale;
   DeviceGuard on(ctx->device);
   cudaStream_t s = stream_of(ctx, stream);
-  const unsigned grid = (unsigned)std::min<uint64_t>(a.g.rows, kMaxGrid);
-  if (dlogits) launch<true>(a, logits->dtype, grid, s);
-  else launch<false>(a, logits->dtype, grid, s);
-  return launched(ctx, dlogits ? "distill_grad_strided" : "distill_loss_strided");
+  const bool unit = a.vocab == 1 || (a.x.inner == 1 && (!dlogits || a.dx.inner == 1));
+  const cudaError_t e = dlogits ? launch<true>(ctx, a, logits->dtype, unit, s) : launch<false>(ctx, a, logits->dtype, unit, s);
+  if (e != cudaSuccess) return cuda_fail(e, op);
+  return launched(ctx, dlogits ? (unit ? "distill_grad_rows" : "distill_grad_strided")
+                               : (unit ? "distill_loss_rows" : "distill_loss_strided"));
 }
 
 }  // namespace

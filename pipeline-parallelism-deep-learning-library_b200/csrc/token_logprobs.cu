@@ -592,10 +592,10 @@ __global__ void __launch_bounds__(kGradThreads, 4) token_logprobs_backward_rows(
     const Span span = span_of<DT>(dx, a.vocab);
     const char* xv = reinterpret_cast<const char*>(x + span.head);  // where vector 0 of dx reads
     uint4* dv = reinterpret_cast<uint4*>(dx + span.head);
-    const uint32_t shift = MOVED ? reinterpret_cast<uintptr_t>(xv) & 15 : 0;
+    const uint32_t shift = reinterpret_cast<uintptr_t>(xv) & 15;
     // the aligned vectors of x that begin and end within the row, where vector v is cut out of v and v + 1
-    const uint32_t first = MOVED && xv - shift < reinterpret_cast<const char*>(x) ? 1 : 0;
-    const uint32_t count = MOVED ? (uint32_t)((reinterpret_cast<const char*>(x + a.vocab) - (xv - shift)) / 16) : 0;
+    const uint32_t first = xv - shift < reinterpret_cast<const char*>(x);
+    const uint32_t count = (uint32_t)((reinterpret_cast<const char*>(x + a.vocab) - (xv - shift)) / 16);
     const uint32_t step = kU * blockDim.x;
     const uint32_t from = min(span.vecs, tile * steps * step), to = min(span.vecs, from + steps * step);
     bool ready = false;

@@ -14,7 +14,6 @@
 // form is e^(scale (x_j - mt)) (c e^(scale (mt - m)) / S - r / St), which stands also where Q underflows.
 #include <cmath>
 
-#include "ptx.cuh"
 #include "vocab.cuh"
 
 namespace {
@@ -206,19 +205,14 @@ __global__ void __launch_bounds__(kThreads) distill_strided(DistillArgs a) {
 
 // ---- the vocabulary as the unit axis -----------------------------------------------------------
 //
-// A cluster of blocks a row, each with a slice of it in shared memory: the copy engine brings the slice in while the block
-// works out the teacher's list, the list's places in it are set to minus infinity, and the sums and the gradient are two
-// passes over shared memory.  So a row crosses HBM once each way.  Between the passes the blocks tell one another their sums.
-// A slice that does not fit comes in chunks, once for each pass.
-constexpr int kRowThreads = 256;
-constexpr int kUnroll = 4;
+// One block a row, or a cluster of blocks where there are few rows, each with a slice.  Two passes over the slice: the sums,
+// in which a bit for each place tells the list's places, and the gradient.  Between them the blocks of a cluster tell one
+// another their sums.  The second pass finds the row in L2, so it crosses HBM once each way.
+template <int DT>
+constexpr int kUnroll = 32 / Vec<DT>::kElems;  // vectors of a step: 32 places a thread
+constexpr int kRowThreads = 512;
 constexpr uint32_t kMaxCluster = 8;
-
-// What a block tells the others of its cluster.
-struct Part {
-  float rest_m, rest_s, named_m, named_s;
-  double p, dot;  // sum P and sum P scale (x - named_m) over the list's places in the slice
-};
+constexpr uint64_t kMaxBits = 64 << 10;  // bytes of shared memory for a slice's bits
 
 // A thread's entry of the list.
 struct Entry {
@@ -226,57 +220,81 @@ struct Entry {
   double p;     // 64 bits: the loss has sum P scale x beside sum P log P, which cancel to a small part
 };
 
-__device__ __forceinline__ double2 block_sum(double2 v, double2* red) {
+// The teacher's list and the student's logits at its places are worked out by the first `warps` warps, an entry a thread,
+// while the others go on with the row.
+__device__ __forceinline__ void list_sync(uint32_t warps) {
+  if (warps > 1) asm volatile("bar.sync 1, %0;" ::"r"(warps * 32) : "memory");
+  else __syncwarp();
+}
+
+struct Said {
+  double sum, plogp;  // sum P and sum P log P over the entries that stand
+  Soft named;         // the student's logits there
+};
+
+struct ListWork {  // shared memory of the list's warps
+  float top[kMaxList / 32];
+  double2 sums[kMaxList / 32];
+  Soft named[kMaxList / 32];
+};
+
+__device__ __forceinline__ double2 warp_sum(double2 v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
     v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
   }
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x / 32] = v;
-  __syncthreads();
-  v = red[0];
-  for (int w = 1; w < (int)blockDim.x / 32; w++) v = make_double2(v.x + red[w].x, v.y + red[w].y);
-  __syncthreads();
   return v;
 }
 
-// The teacher's list of row r, an entry a thread; `sums`: sum P and sum P log P.
-__device__ __forceinline__ Entry read_entry(const DistillArgs& a, uint64_t r, uint32_t* ids, float* redf, double2* redd, double2* sums) {
-  const uint32_t k = threadIdx.x;
-  const bool here = k < a.list;
-  Entry e{0xffffffffu, 0.0};
-  float z = neg_inf();
-  if (here) {
-    e.id = static_cast<const uint32_t*>(a.ids.data)[row_at(a.g, a.ids, r) + k * a.ids.inner];
-    z = teacher_value(a, row_at(a.g, a.teacher, r) + k * a.teacher.inner);
-    ids[k] = e.id;
+// Called by the list's warps: drops this thread's entry if an earlier one names the same place, weighs it, and leaves in
+// `said` what the whole list says.  `xk`: the student's logit at the entry's place.
+__device__ __forceinline__ void weigh(const DistillArgs& a, const uint32_t* ids, float z, float* xk, Entry* entry, uint32_t warps,
+                                      float c2, ListWork* work, Said* said) {
+  Entry e = *entry;
+  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  if (e.id != 0xffffffffu) {
+    bool again = false;
+    for (uint32_t i = 0; i < threadIdx.x; i++) again |= ids[i] == e.id;
+    if (again) e.id = 0xffffffffu;
   }
-  __syncthreads();
-  bool stands = here && e.id < a.vocab;
-  if (stands)
-    for (uint32_t i = 0; i < k; i++) stands = stands && ids[i] != e.id;
-  if (!stands) {
-    e.id = 0xffffffffu;
-    z = neg_inf();
-  }
+  if (e.id == 0xffffffffu) z = *xk = neg_inf();
   double lz = z, w = 0.0;
   if (!a.tail) {
-    const float top = base_of(block_max(z, redf));
-    lz = (double)a.scale * ((double)z - (double)top);
+    float top = warp_top(z);
+    if (warps > 1) {
+      if (lane == 0) work->top[warp] = top;
+      list_sync(warps);
+      top = warp_top(lane < warps ? work->top[lane] : neg_inf());
+    }
+    lz = (double)a.scale * ((double)z - (double)base_of(top));
   }
-  if (stands) w = exp(lz);
-  // of the renormalised P = w / total: sum P log P = (sum w lz) / total - log total
-  const double2 t = block_sum(make_double2(w, w > 0.0 || isnan(w) ? w * lz : 0.0), redd);
-  if (a.tail) {
-    *sums = t;
-    e.p = w;
-  } else if (t.x > 0.0 || isnan(t.x)) {
-    *sums = make_double2(isnan(t.x) ? t.x : 1.0, t.y / t.x - log(t.x));
-    e.p = w / t.x;
-  } else {  // no entry says anything
-    *sums = make_double2(0.0, 0.0);
+  if (e.id != 0xffffffffu) w = exp(lz);
+  double2 t = warp_sum(make_double2(w, w > 0.0 || isnan(w) ? w * lz : 0.0));
+  Soft named = warp_merge(Soft{*xk, *xk == neg_inf() ? 0.0f : 1.0f, 0.0f}, c2);
+  if (warps > 1) {
+    if (lane == 0) {
+      work->sums[warp] = t;
+      work->named[warp] = named;
+    }
+    list_sync(warps);
+    t = warp_sum(lane < warps ? work->sums[lane] : make_double2(0.0, 0.0));
+    named = warp_merge(lane < warps ? work->named[lane] : Soft{neg_inf(), 0.0f, 0.0f}, c2);
   }
-  return e;
+  e.p = w;
+  double sum = t.x, plogp = t.y;
+  if (!a.tail) {
+    // of the renormalised P = w / total: sum P log P = (sum w lz) / total - log total
+    if (t.x > 0.0 || isnan(t.x)) {
+      e.p = w / t.x;
+      sum = isnan(t.x) ? t.x : 1.0;
+      plogp = t.y / t.x - log(t.x);
+    } else {  // no entry says anything
+      e.p = sum = plogp = 0.0;
+    }
+  }
+  if (threadIdx.x == 0) *said = Said{sum, plogp, named};
+  *entry = e;
 }
 
 // dx = coef 2^d outside the list, in the same two forms of d as take (vocab.cuh)
@@ -306,28 +324,39 @@ __device__ __forceinline__ float tail_of(float x, const Tail& w, float c2) {
   return ex2(w.wide ? (x + w.minus) * c2 : __fmaf_rn(x, c2, w.minus)) * w.coef;
 }
 
-// chunk: vectors of shared memory; chunks: how many a slice takes.
+// `bits` say which places of a vector are the list's: they become minus infinity.
+template <int DT>
+__device__ __forceinline__ void take_out(uint4& q, uint32_t bits) {
+  uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if constexpr (DT == LC_F32) {
+      if (bits >> i & 1) w[i] = 0xff800000u;
+    } else {
+      const uint32_t inf = DT == LC_F16 ? 0xfc00u : 0xff80u;
+      if (bits >> (2 * i) & 1) w[i] = (w[i] & 0xffff0000u) | inf;
+      if (bits >> (2 * i + 1) & 1) w[i] = (w[i] & 0xffffu) | inf << 16;
+    }
+  }
+  q = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A place's byte and bit: a byte a vector (of f32 four bits are used).
 template <int DT, bool GRAD, bool MOVED>
-__global__ void __launch_bounds__(kRowThreads, 5) distill_rows(DistillArgs a, uint32_t cluster, uint32_t share, uint32_t chunk, int* err) {
+__global__ void __launch_bounds__(kRowThreads, 3) distill_rows(DistillArgs a, uint32_t cluster, uint32_t share) {
   using E = Elem<DT>;
   using T = typename E::T;
   constexpr uint32_t kE = Vec<DT>::kElems;
-  extern __shared__ __align__(128) uint4 data[];  // [chunk], and 16 bytes more
-  __shared__ uint64_t full;
+  constexpr int kU = kUnroll<DT>;
+  extern __shared__ __align__(16) uint8_t in_list[];  // [share], a multiple of 16
   __shared__ uint32_t ids[kMaxList];
-  __shared__ Soft red[2][kRowThreads / 32];
-  __shared__ float redf[kRowThreads / 32], edges[16];
-  __shared__ double2 redd[kRowThreads / 32];
-  __shared__ Part parts[kMaxCluster];
-  T* const in = reinterpret_cast<T*>(data);
-  const uint32_t rank = cluster > 1 ? cluster_rank() : 0;
+  __shared__ Soft red[kRowThreads / 32];
+  __shared__ float edges[16];
+  __shared__ ListWork work;
+  __shared__ Said said;
+  __shared__ float2 parts[kMaxCluster];  // (m, s) of the places outside the list, from each block of the cluster
+  const uint32_t rank = cluster > 1 ? cluster_rank() : 0, list_warps = max(1u, (a.list + 31) / 32);
   const float c2 = a.scale * kLog2e;
-  if (threadIdx.x == 0) {
-    lcd::mbar_init(&full, 1);
-    lcd::fence_mbar_init();
-  }
-  __syncthreads();
-  uint32_t parity = 0;
   // Cluster barriers alternate: every block's `parts` are free (at first: it has started), and they are filled.
   if (cluster > 1) cluster_arrive();
   for (uint64_t r = blockIdx.x / cluster; r < a.g.rows; r += gridDim.x / cluster) {
@@ -335,15 +364,15 @@ __global__ void __launch_bounds__(kRowThreads, 5) distill_rows(DistillArgs a, ui
     const Span span = span_of<DT>(x, a.vocab);
     const uint32_t from = min(span.vecs, rank * share), to = min(span.vecs, from + share);
     const uint4* vec = reinterpret_cast<const uint4*>(x + span.head);
-    auto fetch = [&](uint32_t v0) {  // vectors v0 .. of the slice; the last reads of shared memory are behind a barrier
-      if (threadIdx.x == 0) {
-        lcd::fence_proxy_async_smem();
-        const uint32_t n = min(chunk, to - v0);
-        lcd::mbar_arrive_expect_tx(&full, n * 16);
-        copy_in(data, vec + v0, n * 16, &full);
-      }
-    };
-    if (from < to) fetch(from);
+    Entry entry{0xffffffffu, 0.0};
+    float z = neg_inf(), xk = neg_inf();
+    if (threadIdx.x < a.list) {
+      entry.id = static_cast<const uint32_t*>(a.ids.data)[row_at(a.g, a.ids, r) + threadIdx.x * a.ids.inner];
+      z = teacher_value(a, row_at(a.g, a.teacher, r) + threadIdx.x * a.teacher.inner);
+      ids[threadIdx.x] = entry.id;
+      if (entry.id < a.vocab) xk = E::up(x[entry.id]);
+      else entry.id = 0xffffffffu;
+    }
     // the places before the vectors (0-7) and behind them (8-15) are block 0's
     uint32_t edge_at = 0xffffffffu;
     if (rank == 0 && threadIdx.x < 16) {
@@ -353,105 +382,86 @@ __global__ void __launch_bounds__(kRowThreads, 5) distill_rows(DistillArgs a, ui
         edges[threadIdx.x] = E::up(x[edge_at]);
       }
     }
+    for (uint32_t i = threadIdx.x; i < (to - from + 15) / 16; i += blockDim.x) reinterpret_cast<uint4*>(in_list)[i] = make_uint4(0, 0, 0, 0);
     const float d_loss = GRAD && a.d_loss.data ? static_cast<const float*>(a.d_loss.data)[row_at(a.g, a.d_loss, r)] : 1.0f;
-    double2 sums;
-    const Entry entry = read_entry(a, r, ids, redf, redd, &sums);
-    // where the entry's place lies: in the vectors (counted in places from the first of them), or among the edges
-    const uint32_t at = entry.id - span.head;
-    const bool in_vecs = entry.id != 0xffffffffu && entry.id >= span.head && at < span.vecs * kE;
-    float xk = neg_inf();
+    __syncthreads();
+    // where the entry's place lies: in the slice's vectors, or among the edges
     bool mine = false;
-    if (rank == 0 && entry.id != 0xffffffffu && !in_vecs) {
-      float* e = &edges[entry.id < span.head ? entry.id : 8 + at - span.vecs * kE];
-      xk = *e;
-      *e = neg_inf();
-      mine = true;
-    }
-    // takes the list's places out of the chunk that begins with vector v0
-    auto mark = [&](uint32_t v0, uint32_t n) {
-      if (in_vecs && at >= v0 * kE && at < (v0 + n) * kE) {
-        xk = E::up(in[at - v0 * kE]);
-        in[at - v0 * kE] = E::down(neg_inf());
+    if (entry.id != 0xffffffffu) {
+      const uint32_t at = entry.id - span.head, v = at / kE;
+      if (entry.id >= span.head && at < span.vecs * kE) {
+        mine = v >= from && v < to;
+        if (mine) atomicOr(reinterpret_cast<uint32_t*>(in_list) + (v - from) / 4, 1u << ((v - from) % 4 * 8 + at % kE));
+      } else if (rank == 0) {
+        edges[entry.id < span.head ? entry.id : 8 + at - span.vecs * kE] = neg_inf();
         mine = true;
       }
-    };
+    }
+    __syncthreads();
+    if (threadIdx.x / 32 < list_warps) weigh(a, ids, z, &xk, &entry, list_warps, c2, &work, &said);
+    mine = mine && entry.id != 0xffffffffu;
     Run run = empty_run();
-    for (uint32_t v0 = from; v0 < to; v0 += chunk) {
-      if (v0 > from) {
-        __syncthreads();
-        fetch(v0);
-      }
-      const uint32_t n = min(chunk, to - v0);
-      lcd::mbar_wait(&full, parity, err);
-      parity ^= 1;
-      mark(v0, n);
-      __syncthreads();
-      uint32_t i = threadIdx.x;
-      for (; i + (kUnroll - 1) * blockDim.x < n; i += kUnroll * blockDim.x) {
-        uint4 q[kUnroll];
+    {
+      const uint32_t step = kU * blockDim.x;
+      const uint8_t* bits = in_list - from;
+      uint32_t v0 = from;
+      for (; v0 + step <= to; v0 += step) {
+        uint4 q[kU];
+        uint32_t m[kU], any = 0;
 #pragma unroll
-        for (int u = 0; u < kUnroll; u++) q[u] = data[i + u * blockDim.x];
+        for (int u = 0; u < kU; u++) q[u] = __ldg(vec + v0 + u * blockDim.x + threadIdx.x);
+#pragma unroll
+        for (int u = 0; u < kU; u++) any |= m[u] = bits[v0 + u * blockDim.x + threadIdx.x];
+        if (any) {
+#pragma unroll
+          for (int u = 0; u < kU; u++) take_out<DT>(q[u], m[u]);
+        }
         float top = Vec<DT>::top(q[0]);
 #pragma unroll
-        for (int u = 1; u < kUnroll; u++) top = max_nan(top, Vec<DT>::top(q[u]));
-        take<DT, kUnroll, false>(run, q, top, c2);
+        for (int u = 1; u < kU; u++) top = max_nan(top, Vec<DT>::top(q[u]));
+        take<DT, kU, false>(run, q, top, c2);
       }
-      for (; i < n; i += blockDim.x) {
-        const uint4 q[1] = {data[i]};
-        take<DT, 1, false>(run, q, Vec<DT>::top(q[0]), c2);
+      if (v0 < to) {
+        uint4 q[kU][1];
+#pragma unroll
+        for (int u = 0; u < kU; u++) {
+          const uint32_t v = v0 + u * blockDim.x + threadIdx.x;
+          if (v < to) q[u][0] = __ldg(vec + v);
+        }
+#pragma unroll
+        for (int u = 0; u < kU; u++) {
+          const uint32_t v = v0 + u * blockDim.x + threadIdx.x;
+          if (v >= to) break;
+          take_out<DT>(q[u][0], bits[v]);
+          take<DT, 1, false>(run, q[u], Vec<DT>::top(q[u][0]), c2);
+        }
       }
     }
-    if (from == to) __syncthreads();  // the edges are written and marked
     Soft rest = soft_of(run, c2);
     if (edge_at != 0xffffffffu) {
       const float e = edges[threadIdx.x];
       rest = merge(rest, Soft{e, e == neg_inf() ? 0.0f : 1.0f, 0.0f}, c2);
     }
-    rest = block_merge(rest, c2, red[0]);
-    Soft named = block_merge(Soft{xk, xk == neg_inf() ? 0.0f : 1.0f, 0.0f}, c2, red[1]);
-    // P > 0 at a masked place makes the loss infinite; P = 0 there says nothing
-    const bool says = mine && entry.p != 0.0;
-    const double2 dots = block_sum(
-        says ? make_double2(entry.p, entry.p * ((double)a.scale * ((double)xk - (double)base_of(named.m)))) : make_double2(0.0, 0.0), redd);
+    rest = block_merge(rest, c2, red);  // its barrier is also that of `said`
+    const Soft named = said.named;
     if (cluster > 1) {
       cluster_wait();
       if (threadIdx.x < cluster) {
         const uint32_t to_part = remote(&parts[rank], threadIdx.x);
-        store_remote(to_part, (uint64_t)__float_as_uint(rest.m) | (uint64_t)__float_as_uint(rest.s) << 32);
-        store_remote(to_part + 8, (uint64_t)__float_as_uint(named.m) | (uint64_t)__float_as_uint(named.s) << 32);
-        store_remote(to_part + 16, (uint64_t)__double_as_longlong(dots.x));
-        store_remote(to_part + 24, (uint64_t)__double_as_longlong(dots.y));
+        store_remote(to_part, rest.m);
+        store_remote(to_part + 4, rest.s);
       }
       cluster_arrive();
       cluster_wait();
-      rest = named = Soft{neg_inf(), 0.0f, 0.0f};
-      for (uint32_t c = 0; c < cluster; c++) {
-        rest = merge(rest, Soft{parts[c].rest_m, parts[c].rest_s, 0.0f}, c2);
-        named = merge(named, Soft{parts[c].named_m, parts[c].named_s, 0.0f}, c2);
-      }
+      const uint32_t lane = threadIdx.x & 31;
+      rest = warp_merge(lane < cluster ? Soft{parts[lane].x, parts[lane].y, 0.0f} : Soft{neg_inf(), 0.0f, 0.0f}, c2);
+      cluster_arrive();
     }
     const Soft all = merge(rest, named, c2);
-    // sum P scale (x - m) over the whole list
-    auto from_top = [&](double p, double d, float m) { return d + p * ((double)a.scale * ((double)base_of(m) - (double)base_of(all.m))); };
-    double dot;
-    if (cluster > 1) {
-      dot = 0.0;
-      for (uint32_t c = 0; c < cluster; c++) dot += from_top(parts[c].p, parts[c].dot, parts[c].named_m);
-      cluster_arrive();
-    } else {
-      dot = from_top(dots.x, dots.y, named.m);
-    }
-    double left = a.tail ? 1.0 - sums.x : 0.0;
+    double left = a.tail ? 1.0 - said.sum : 0.0;
     if (left < 0.0 || rest.s == 0.0f) left = 0.0;
-    const float total = (float)(sums.x + left), tail = (float)left;
+    const float total = (float)(said.sum + left), tail = (float)left;
     const float lead = (base_of(rest.m) - base_of(all.m)) * a.scale;  // at most 0 where it counts
-    if (a.loss.data && rank == 0 && threadIdx.x == 0) {
-      // sum P (log P - log q) with log q = scale (x - m) - log S
-      double loss = sums.y - (dot - sums.x * (double)logf(all.s));
-      if (all.s == 0.0f) loss = sums.x > 0.0 ? (double)__int_as_float(0x7f800000) : 0.0;
-      if (tail > 0.0f) loss += (double)(tail * (logf(tail) - (logf(rest.s) + lead - logf(all.s))));
-      static_cast<float*>(a.loss.data)[row_at(a.g, a.loss, r)] = (float)loss;
-    }
     if constexpr (GRAD) {
       float weight = d_loss * a.scale;
       // against mc / c2, which is where 2^d is taken from (vocab.cuh)
@@ -463,41 +473,82 @@ __global__ void __launch_bounds__(kRowThreads, 5) distill_rows(DistillArgs a, ui
       const float in_coef = all.s == 0.0f ? 0.0f : total / all.s * weight;
       if (all.m == neg_inf()) weight = 0.0f;  // masked throughout: there is no distribution, and no gradient
       T* dx = static_cast<T*>(a.dx.data) + row_at(a.g, a.dx, r);
-      for (uint32_t v0 = from; v0 < to; v0 += chunk) {
-        const uint32_t n = min(chunk, to - v0);
-        if (to - from > chunk) {  // the slice's other chunks have been here since
-          __syncthreads();
-          fetch(v0);
-          lcd::mbar_wait(&full, parity, err);
-          parity ^= 1;
-          mark(v0, n);
-          __syncthreads();
+      if constexpr (!MOVED) {
+        uint4* const dv = reinterpret_cast<uint4*>(dx + span.head);
+        const uint32_t step = 4 * blockDim.x;
+        uint32_t v0 = from + threadIdx.x;
+        for (; v0 + 3 * blockDim.x < to; v0 += step) {
+          uint4 q[4];
+#pragma unroll
+          for (int u = 0; u < 4; u++) q[u] = vec[v0 + u * blockDim.x];
+#pragma unroll
+          for (int u = 0; u < 4; u++) __stcs(dv + v0 + u * blockDim.x, tail_vec<DT>(q[u], w, c2));
         }
-        T* const out = dx + span.head + (uint64_t)v0 * kE;
-        if constexpr (!MOVED) {
-          uint4* const ov = reinterpret_cast<uint4*>(out);
-#pragma unroll 4
-          for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) __stcs(ov + i, tail_vec<DT>(data[i], w, c2));
-        } else {
-          // whole vectors of dx, cut out of shared memory; the places around them one by one
-          const Span os = span_of<DT>(out, n * kE);
-          uint4* const ov = reinterpret_cast<uint4*>(out + os.head);
-          const uint32_t shift = os.head * (16 / kE);
-#pragma unroll 4
-          for (uint32_t i = threadIdx.x; i < os.vecs; i += blockDim.x)
-            __stcs(ov + i, tail_vec<DT>(shifted(data[i], data[i + 1], shift), w, c2));
-          if (threadIdx.x < 16) {
-            const uint32_t i = threadIdx.x & 7;
-            if (threadIdx.x < 8 ? i < os.head : i < os.tail) {
-              const uint32_t j = threadIdx.x < 8 ? i : os.head + os.vecs * kE + i;
-              out[j] = E::down(tail_of(E::up(in[j]), w, c2));
-            }
+        if (v0 < to) {
+          uint4 q[4];
+#pragma unroll
+          for (int u = 0; u < 4; u++)
+            if (v0 + u * blockDim.x < to) q[u] = vec[v0 + u * blockDim.x];
+#pragma unroll
+          for (int u = 0; u < 4; u++)
+            if (v0 + u * blockDim.x < to) __stcs(dv + v0 + u * blockDim.x, tail_vec<DT>(q[u], w, c2));
+        }
+      } else {
+        // the slice's places, as whole vectors of dx: each is cut out of two aligned ones of x, of which the second comes
+        // from the next lane
+        const uint32_t places = (to - from) * kE, lane = threadIdx.x & 31;
+        T* const out = dx + span.head + from * kE;
+        const Span os = span_of<DT>(out, places);
+        const uint32_t shift = os.head * (16 / kE);
+        uint4* const dv = reinterpret_cast<uint4*>(out + os.head);
+        const uint4* const xa = vec + from;  // vector i of dx is cut out of i and i + 1
+        for (uint32_t v0 = (threadIdx.x & ~31u) * 4; v0 < os.vecs; v0 += 4 * blockDim.x) {
+          uint4 q[4], last = make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int u = 0; u < 4; u++) {
+            const uint32_t v = v0 + u * 32 + lane;
+            q[u] = v < to - from ? __ldg(xa + v) : make_uint4(0, 0, 0, 0);
+          }
+          if (lane == 31 && v0 + 128 < to - from) last = __ldg(xa + v0 + 128);
+#pragma unroll
+          for (int u = 0; u < 4; u++) {
+            uint4 give = q[u];
+            if (u + 1 < 4 && lane == 0) give = q[u + 1 < 4 ? u + 1 : u];
+            uint4 next = make_uint4(__shfl_sync(0xffffffffu, give.x, lane + 1), __shfl_sync(0xffffffffu, give.y, lane + 1),
+                                    __shfl_sync(0xffffffffu, give.z, lane + 1), __shfl_sync(0xffffffffu, give.w, lane + 1));
+            if (u + 1 == 4 && lane == 31) next = last;
+            const uint32_t v = v0 + u * 32 + lane;
+            if (v < os.vecs) __stcs(dv + v, tail_vec<DT>(shifted(q[u], next, shift), w, c2));
+          }
+        }
+        if (threadIdx.x < 16) {
+          const uint32_t i = threadIdx.x & 7;
+          if (threadIdx.x < 8 ? i < os.head : i < os.tail) {
+            const uint32_t j = threadIdx.x < 8 ? i : os.head + os.vecs * kE + i;
+            out[j] = E::down(tail_of(E::up(x[span.head + from * kE + j]), w, c2));
           }
         }
       }
       if (edge_at != 0xffffffffu) dx[edge_at] = E::down(tail_of(edges[threadIdx.x], w, c2));
-      __syncthreads();
+      __syncthreads();  // the list's places come last
       if (mine) dx[entry.id] = E::down(ex2((xk - base_of(all.m)) * c2) * in_coef - weight * (float)entry.p);
+    }
+    if (a.loss.data && rank == 0 && threadIdx.x / 32 < list_warps) {
+      // sum P (log P - log q) with log q = scale (x - m) - log S; P > 0 at a masked place makes it infinite, P = 0 says nothing
+      const bool says = entry.p != 0.0 && entry.id != 0xffffffffu;
+      double2 dot = make_double2(says ? entry.p * ((double)a.scale * ((double)xk - (double)base_of(all.m))) : 0.0, 0.0);
+      dot = warp_sum(dot);
+      if (list_warps > 1) {
+        if ((threadIdx.x & 31) == 0) work.sums[threadIdx.x / 32] = dot;
+        list_sync(list_warps);
+        if (threadIdx.x < 32) dot = warp_sum(threadIdx.x < list_warps ? work.sums[threadIdx.x] : make_double2(0.0, 0.0));
+      }
+      if (threadIdx.x == 0) {
+        double loss = said.plogp - (dot.x - said.sum * (double)logf(all.s));
+        if (all.s == 0.0f) loss = said.sum > 0.0 ? (double)__int_as_float(0x7f800000) : 0.0;
+        if (tail > 0.0f) loss += (double)(tail * (logf(tail) - (logf(rest.s) + lead - logf(all.s))));
+        static_cast<float*>(a.loss.data)[row_at(a.g, a.loss, r)] = (float)loss;
+      }
     }
     __syncthreads();
   }
@@ -511,27 +562,20 @@ lc_status launched(lc_context* ctx, const char* name) {
   return LC_OK;
 }
 
-// Slices of 32 KB, so that several blocks share an SM and one computes while another waits for its slice or stores; smaller
-// ones where there are few rows.  Up to 96 KB of a slice is held at once.
-constexpr uint64_t kSlice = 32 << 10, kSmallSlice = 8 << 10, kHeld = 96 << 10;
-
+// A cluster for rows that are few, or so long that their bits would not fit in shared memory.
 template <int DT, bool GRAD>
-cudaError_t launch_rows(const lc_context* ctx, const DistillArgs& a, cudaStream_t stream) {
+cudaError_t launch_rows(const lc_context* ctx, const DistillArgs& a, uint32_t cluster, cudaStream_t stream) {
   constexpr uint64_t kE = Vec<DT>::kElems;
   const uint64_t vecs = a.vocab / kE;
-  uint32_t cluster = 1;
-  while (cluster < kMaxCluster && (vecs * 16 > kSlice * cluster ||
-                                   (a.g.rows * cluster < 2ull * ctx->sm_count && vecs * 16 > kSmallSlice * cluster)))
-    cluster *= 2;
-  const uint64_t share = std::max<uint64_t>(1, (vecs + cluster - 1) / cluster), chunk = std::min<uint64_t>(share, kHeld / 16);
-  const uint64_t busy = std::max<uint64_t>((chunk + kUnroll - 1) / kUnroll, a.list);
+  const uint64_t share = std::max<uint64_t>(16, ((vecs + cluster - 1) / cluster + 15) / 16 * 16);
+  const uint64_t busy = std::max<uint64_t>((share + kUnroll<DT> - 1) / kUnroll<DT>, a.list);
   const uint32_t threads = (uint32_t)std::min<uint64_t>(kRowThreads, std::max<uint64_t>(32, (busy + 31) / 32 * 32));
   const bool moved = GRAD && apart(a.g, a.x, a.dx, 16 / kE);
-  void (*kernel)(DistillArgs, uint32_t, uint32_t, uint32_t, int*) = moved ? distill_rows<DT, GRAD, GRAD> : distill_rows<DT, GRAD, false>;
+  void (*kernel)(DistillArgs, uint32_t, uint32_t) = moved ? distill_rows<DT, GRAD, GRAD> : distill_rows<DT, GRAD, false>;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(std::min<uint64_t>(a.g.rows, kMaxGrid) * cluster));
   cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = (chunk + 1) * 16;
+  cfg.dynamicSmemBytes = share;
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -539,14 +583,24 @@ cudaError_t launch_rows(const lc_context* ctx, const DistillArgs& a, cudaStream_
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = cluster > 1 ? 1 : 0;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes);
-  if (e != cudaSuccess) return e;
-  return cudaLaunchKernelEx(&cfg, kernel, a, cluster, (uint32_t)share, (uint32_t)chunk, ctx->d_error);
+  if (cfg.dynamicSmemBytes > (40 << 10)) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaLaunchKernelEx(&cfg, kernel, a, cluster, (uint32_t)share);
+}
+
+uint32_t cluster_of(const lc_context* ctx, uint64_t rows, uint64_t vecs) {
+  uint32_t cluster = 1;
+  while (cluster < kMaxCluster && (vecs > kMaxBits * cluster || (rows * cluster < 2ull * ctx->sm_count && vecs > 1024ull * cluster)))
+    cluster *= 2;
+  return cluster;
 }
 
 template <int DT, bool GRAD>
 cudaError_t launch(const lc_context* ctx, const DistillArgs& a, bool unit, cudaStream_t stream) {
-  if (unit) return launch_rows<DT, GRAD>(ctx, a, stream);
+  const uint64_t vecs = a.vocab / Vec<DT>::kElems;
+  if (unit && vecs <= (kMaxBits - 16) * kMaxCluster) return launch_rows<DT, GRAD>(ctx, a, cluster_of(ctx, a.g.rows, vecs), stream);
   distill_strided<DT, GRAD><<<(unsigned)std::min<uint64_t>(a.g.rows, kMaxGrid), kThreads, 0, stream>>>(a);
   return cudaSuccess;
 }

@@ -153,6 +153,26 @@ __device__ __forceinline__ uint4 one_by_one(const void* at) {
   }
 }
 
+// 16 bytes with an L2 policy: kept for a second pass, or let go after it
+__device__ __forceinline__ uint64_t keep_in_l2() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_last.b64 %0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ uint64_t leave_l2() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ uint4 load_with(const void* p, uint64_t policy) {
+  uint4 q;
+  asm volatile("ld.global.L1::no_allocate.L2::cache_hint.v4.u32 {%0, %1, %2, %3}, [%4], %5;"
+               : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
+               : "l"(p), "l"(policy)
+               : "memory");
+  return q;
+}
+
 struct Soft {
   float m, s, t;
 };

@@ -212,7 +212,10 @@ template <int DT>
 constexpr int kUnroll = 32 / Vec<DT>::kElems;  // vectors of a step: 32 places a thread
 template <bool GRAD>
 constexpr int kRowThreads = GRAD ? 512 : 256;
+template <int DT, bool GRAD>
+constexpr int kResident = GRAD ? 2 : DT == LC_F32 ? 4 : 6;  // blocks an SM
 constexpr uint32_t kMaxCluster = 8;
+constexpr uint64_t kLongSlice = 128 << 10;  // bytes
 constexpr uint64_t kMaxBits = 64 << 10;  // bytes of shared memory for a slice's bits
 
 // A thread's entry of the list.
@@ -342,98 +345,66 @@ __device__ __forceinline__ void take_out(uint4& q, uint32_t bits) {
   q = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// The list's warps are a row ahead: while the others begin the gradient of a row they work out the next row's list, whose
-// loads depend on one another, and then join; the gradient's tiles go to whichever warp is free.  (Its places do not depend
-// on one another; the sums' do, and their order does not vary.)
+// A place's byte and bit: a byte a vector (of f32 four bits are used).
 template <int DT, bool GRAD, bool MOVED>
-__global__ void __launch_bounds__(kRowThreads<GRAD>, GRAD ? 2 : 5) distill_rows(DistillArgs a, uint32_t cluster, uint32_t share) {
+__global__ void __launch_bounds__(kRowThreads<GRAD>, kResident<DT, GRAD>) distill_rows(DistillArgs a, uint32_t cluster, uint32_t share) {
   using E = Elem<DT>;
   using T = typename E::T;
   constexpr uint32_t kE = Vec<DT>::kElems;
   constexpr int kU = kUnroll<DT>;
-  extern __shared__ __align__(16) uint8_t in_list[];  // [share], a multiple of 16: a byte a vector, a bit a place
+  extern __shared__ __align__(16) uint8_t in_list[];  // [share], a multiple of 16
   __shared__ uint32_t ids[kMaxList];
   __shared__ Soft red[kRowThreads<GRAD> / 32];
+  __shared__ float edges[16];
   __shared__ ListWork work;
-  __shared__ Said said[2];
-  __shared__ uint32_t edge_in_list, next_tile;
+  __shared__ Said said;
   __shared__ float2 parts[kMaxCluster];  // (m, s) of the places outside the list, from each block of the cluster
-  const uint32_t rank = cluster > 1 ? cluster_rank() : 0, list_warps = max(1u, (a.list + 31) / 32), lane = threadIdx.x & 31;
-  const bool lists = threadIdx.x / 32 < list_warps;
+  const uint32_t rank = cluster > 1 ? cluster_rank() : 0, list_warps = max(1u, (a.list + 31) / 32);
   const float c2 = a.scale * kLog2e;
-  const uint64_t keep = keep_in_l2(), leave = leave_l2(), stride = gridDim.x / cluster;
-
-  Entry entry{0xffffffffu, 0.0};
-  float xk = neg_inf();
-  // the list of row r, by its warps
-  auto read_list = [&](uint64_t r, Said* to_said) {
-    const T* x = static_cast<const T*>(a.x.data) + row_at(a.g, a.x, r);
-    Entry e{0xffffffffu, 0.0};
-    float z = neg_inf();
-    xk = neg_inf();
-    if (threadIdx.x < a.list) {
-      e.id = static_cast<const uint32_t*>(a.ids.data)[row_at(a.g, a.ids, r) + threadIdx.x * a.ids.inner];
-      z = teacher_value(a, row_at(a.g, a.teacher, r) + threadIdx.x * a.teacher.inner);
-      ids[threadIdx.x] = e.id;
-      if (e.id < a.vocab) xk = E::up(x[e.id]);
-      else e.id = 0xffffffffu;
-    }
-    list_sync(list_warps);
-    weigh(a, ids, z, &xk, &e, list_warps, c2, &work, to_said);
-    entry = e;
-  };
-  auto clear_bits = [&] {
-    for (uint32_t i = threadIdx.x; i < share / 16; i += blockDim.x) reinterpret_cast<uint4*>(in_list)[i] = make_uint4(0, 0, 0, 0);
-    if (threadIdx.x == 0) edge_in_list = 0;
-  };
-  auto slice = [&](const Span& span, uint32_t* from, uint32_t* to) {
-    *from = min(span.vecs, rank * share);
-    *to = min(span.vecs, *from + share);
-  };
-  // tells the places of row r that are this thread's entry's; true if they are this block's
-  auto set_bits = [&](uint64_t r) {
-    if (entry.id == 0xffffffffu) return false;
-    const Span span = span_of<DT>(static_cast<const T*>(a.x.data) + row_at(a.g, a.x, r), a.vocab);
-    uint32_t from, to;
-    slice(span, &from, &to);
-    const uint32_t at = entry.id - span.head, v = at / kE;
-    if (entry.id >= span.head && at < span.vecs * kE) {
-      if (v < from || v >= to) return false;
-      atomicOr(reinterpret_cast<uint32_t*>(in_list) + (v - from) / 4, 1u << ((v - from) % 4 * 8 + at % kE));
-      return true;
-    }
-    if (rank == 0) atomicOr(&edge_in_list, 1u << (entry.id < span.head ? entry.id : 8 + at - span.vecs * kE));
-    return rank == 0;
-  };
-
+  const uint64_t keep = keep_in_l2(), leave = leave_l2();
   // Cluster barriers alternate: every block's `parts` are free (at first: it has started), and they are filled.
   if (cluster > 1) cluster_arrive();
-  bool mine = false;
-  uint32_t turn = 0;
-  clear_bits();
-  __syncthreads();
-  if (lists && blockIdx.x / cluster < a.g.rows) {
-    read_list(blockIdx.x / cluster, &said[0]);
-    mine = set_bits(blockIdx.x / cluster);
-  }
-  __syncthreads();
-  for (uint64_t r = blockIdx.x / cluster; r < a.g.rows; r += stride, turn ^= 1) {
+  for (uint64_t r = blockIdx.x / cluster; r < a.g.rows; r += gridDim.x / cluster) {
     const T* x = static_cast<const T*>(a.x.data) + row_at(a.g, a.x, r);
     const Span span = span_of<DT>(x, a.vocab);
-    uint32_t from, to;
-    slice(span, &from, &to);
+    const uint32_t from = min(span.vecs, rank * share), to = min(span.vecs, from + share);
     const uint4* vec = reinterpret_cast<const uint4*>(x + span.head);
-    // the places before the vectors (threads 0-7) and behind them (8-15) are block 0's
+    Entry entry{0xffffffffu, 0.0};
+    float z = neg_inf(), xk = neg_inf();
+    if (threadIdx.x < a.list) {
+      entry.id = static_cast<const uint32_t*>(a.ids.data)[row_at(a.g, a.ids, r) + threadIdx.x * a.ids.inner];
+      z = teacher_value(a, row_at(a.g, a.teacher, r) + threadIdx.x * a.teacher.inner);
+      ids[threadIdx.x] = entry.id;
+      if (entry.id < a.vocab) xk = E::up(x[entry.id]);
+      else entry.id = 0xffffffffu;
+    }
+    // the places before the vectors (0-7) and behind them (8-15) are block 0's
     uint32_t edge_at = 0xffffffffu;
-    float edge = neg_inf();
     if (rank == 0 && threadIdx.x < 16) {
       const uint32_t i = threadIdx.x & 7;
       if (threadIdx.x < 8 ? i < span.head : i < span.tail) {
         edge_at = threadIdx.x < 8 ? i : span.head + span.vecs * kE + i;
-        edge = E::up(x[edge_at]);
+        edges[threadIdx.x] = E::up(x[edge_at]);
       }
     }
+    for (uint32_t i = threadIdx.x; i < (to - from + 15) / 16; i += blockDim.x) reinterpret_cast<uint4*>(in_list)[i] = make_uint4(0, 0, 0, 0);
     const float d_loss = GRAD && a.d_loss.data ? static_cast<const float*>(a.d_loss.data)[row_at(a.g, a.d_loss, r)] : 1.0f;
+    __syncthreads();
+    // where the entry's place lies: in the slice's vectors, or among the edges
+    bool mine = false;
+    if (entry.id != 0xffffffffu) {
+      const uint32_t at = entry.id - span.head, v = at / kE;
+      if (entry.id >= span.head && at < span.vecs * kE) {
+        mine = v >= from && v < to;
+        if (mine) atomicOr(reinterpret_cast<uint32_t*>(in_list) + (v - from) / 4, 1u << ((v - from) % 4 * 8 + at % kE));
+      } else if (rank == 0) {
+        edges[entry.id < span.head ? entry.id : 8 + at - span.vecs * kE] = neg_inf();
+        mine = true;
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x / 32 < list_warps) weigh(a, ids, z, &xk, &entry, list_warps, c2, &work, &said);
+    mine = mine && entry.id != 0xffffffffu;
     Run run = empty_run();
     {
       const uint32_t step = kU * blockDim.x;
@@ -443,10 +414,7 @@ __global__ void __launch_bounds__(kRowThreads<GRAD>, GRAD ? 2 : 5) distill_rows(
         uint4 q[kU];
         uint32_t m[kU], any = 0;
 #pragma unroll
-        for (int u = 0; u < kU; u++) {
-          const uint4* p = vec + v0 + u * blockDim.x + threadIdx.x;
-          q[u] = GRAD ? load_with(p, keep) : load_once(p);
-        }
+        for (int u = 0; u < kU; u++) q[u] = GRAD ? load_with(vec + v0 + u * blockDim.x + threadIdx.x, keep) : load_once(vec + v0 + u * blockDim.x + threadIdx.x);
 #pragma unroll
         for (int u = 0; u < kU; u++) any |= m[u] = bits[v0 + u * blockDim.x + threadIdx.x];
         if (any) {
@@ -476,11 +444,11 @@ __global__ void __launch_bounds__(kRowThreads<GRAD>, GRAD ? 2 : 5) distill_rows(
     }
     Soft rest = soft_of(run, c2);
     if (edge_at != 0xffffffffu) {
-      if (edge_in_list >> threadIdx.x & 1) edge = neg_inf();
-      rest = merge(rest, Soft{edge, edge == neg_inf() ? 0.0f : 1.0f, 0.0f}, c2);
+      const float e = edges[threadIdx.x];
+      rest = merge(rest, Soft{e, e == neg_inf() ? 0.0f : 1.0f, 0.0f}, c2);
     }
-    if (threadIdx.x == 0) next_tile = 0;
-    rest = block_merge(rest, c2, red);
+    rest = block_merge(rest, c2, red);  // its barrier is also that of `said`
+    const Soft named = said.named;
     if (cluster > 1) {
       cluster_wait();
       if (threadIdx.x < cluster) {
@@ -490,69 +458,63 @@ __global__ void __launch_bounds__(kRowThreads<GRAD>, GRAD ? 2 : 5) distill_rows(
       }
       cluster_arrive();
       cluster_wait();
+      const uint32_t lane = threadIdx.x & 31;
       rest = warp_merge(lane < cluster ? Soft{parts[lane].x, parts[lane].y, 0.0f} : Soft{neg_inf(), 0.0f, 0.0f}, c2);
       cluster_arrive();
     }
-    const Soft all = merge(rest, said[turn].named, c2);
-    const double sum = said[turn].sum;
-    double left = a.tail ? 1.0 - sum : 0.0;
+    const Soft all = merge(rest, named, c2);
+    double left = a.tail ? 1.0 - said.sum : 0.0;
     if (left < 0.0 || rest.s == 0.0f) left = 0.0;
-    const float total = (float)(sum + left), tail = (float)left;
+    const float total = (float)(said.sum + left), tail = (float)left;
     const float lead = (base_of(rest.m) - base_of(all.m)) * a.scale;  // at most 0 where it counts
-    const float weight = d_loss * a.scale;
-    clear_bits();  // the row's sums are done with them
-    float own = 0.0f;
-    const Entry now = entry;
-    if (lists) {
-      if constexpr (GRAD) {
-        const float in_coef = all.s == 0.0f ? 0.0f : total / all.s * weight;
-        own = ex2((xk - base_of(all.m)) * c2) * in_coef - (all.m == neg_inf() ? 0.0f : weight) * (float)entry.p;
-      }
-      if (a.loss.data && rank == 0) {
-        // sum P (log P - log q) with log q = scale (x - m) - log S; P > 0 at a masked place makes it infinite, P = 0 says nothing
-        const bool says = entry.p != 0.0 && entry.id != 0xffffffffu;
-        double2 dot = warp_sum(make_double2(says ? entry.p * ((double)a.scale * ((double)xk - (double)base_of(all.m))) : 0.0, 0.0));
-        if (list_warps > 1) {
-          if (lane == 0) work.sums[threadIdx.x / 32] = dot;
-          list_sync(list_warps);
-          if (threadIdx.x < 32) dot = warp_sum(lane < list_warps ? work.sums[lane] : make_double2(0.0, 0.0));
-          list_sync(list_warps);
-        }
-        if (threadIdx.x == 0) {
-          double loss = said[turn].plogp - (dot.x - sum * (double)logf(all.s));
-          if (all.s == 0.0f) loss = sum > 0.0 ? (double)__int_as_float(0x7f800000) : 0.0;
-          if (tail > 0.0f) loss += (double)(tail * (logf(tail) - (logf(rest.s) + lead - logf(all.s))));
-          static_cast<float*>(a.loss.data)[row_at(a.g, a.loss, r)] = (float)loss;
-        }
-      }
-      if (r + stride < a.g.rows) read_list(r + stride, &said[turn ^ 1]);
-    }
-    T* dx = GRAD ? static_cast<T*>(a.dx.data) + row_at(a.g, a.dx, r) : nullptr;
     if constexpr (GRAD) {
+      float weight = d_loss * a.scale;
       // against mc / c2, which is where 2^d is taken from (vocab.cuh)
       Tail w;
       w.wide = is_wide(rest.m, c2);
       w.minus = w.wide ? -base_of(rest.m) : -(rest.m * c2);
       const float off = w.wide ? 0.0f : __fmaf_rn(rest.m, c2, w.minus);
       w.coef = rest.s == 0.0f ? 0.0f : (total * expf(lead) / all.s - tail / rest.s) * weight * ex2(-off);
-      // tiles of 4 vectors a lane, from the end of the slice, which was read last
-      T* const out = dx + span.head + (uint64_t)from * kE;
-      const Span os = span_of<DT>(out, (to - from) * kE);  // the slice's whole vectors of dx
-      uint4* const dv = reinterpret_cast<uint4*>(out + os.head);
-      const uint4* const xa = vec + from;
-      const uint32_t shift = os.head * (16 / kE), tiles = (os.vecs + 127) / 128;
-      for (;;) {
-        uint32_t tile = lane == 0 ? atomicAdd(&next_tile, 1u) : 0;
-        tile = __shfl_sync(0xffffffffu, tile, 0);
-        if (tile >= tiles) break;
-        const uint32_t v0 = (tiles - 1 - tile) * 128 + lane;
-        uint4 q[4];
-        if constexpr (MOVED) {
-          // vector v of dx is cut out of v and v + 1 of x, of which the second comes from the next lane
-          uint4 last = make_uint4(0, 0, 0, 0);
+      const float in_coef = all.s == 0.0f ? 0.0f : total / all.s * weight;
+      if (all.m == neg_inf()) weight = 0.0f;  // masked throughout: there is no distribution, and no gradient
+      T* dx = static_cast<T*>(a.dx.data) + row_at(a.g, a.dx, r);
+      if constexpr (!MOVED) {
+        uint4* const dv = reinterpret_cast<uint4*>(dx + span.head);
+        const uint32_t step = 4 * blockDim.x;
+        uint32_t v0 = from + threadIdx.x;
+        for (; v0 + 3 * blockDim.x < to; v0 += step) {
+          uint4 q[4];
 #pragma unroll
-          for (int u = 0; u < 4; u++) q[u] = v0 + u * 32 < to - from ? load_with(xa + v0 + u * 32, leave) : last;
-          if (lane == 31 && v0 + 97 < to - from) last = load_with(xa + v0 + 97, leave);
+          for (int u = 0; u < 4; u++) q[u] = load_with(vec + v0 + u * blockDim.x, leave);
+#pragma unroll
+          for (int u = 0; u < 4; u++) __stcs(dv + v0 + u * blockDim.x, tail_vec<DT>(q[u], w, c2));
+        }
+        if (v0 < to) {
+          uint4 q[4];
+#pragma unroll
+          for (int u = 0; u < 4; u++)
+            if (v0 + u * blockDim.x < to) q[u] = load_with(vec + v0 + u * blockDim.x, leave);
+#pragma unroll
+          for (int u = 0; u < 4; u++)
+            if (v0 + u * blockDim.x < to) __stcs(dv + v0 + u * blockDim.x, tail_vec<DT>(q[u], w, c2));
+        }
+      } else {
+        // the slice's places, as whole vectors of dx: each is cut out of two aligned ones of x, of which the second comes
+        // from the next lane
+        const uint32_t places = (to - from) * kE, lane = threadIdx.x & 31;
+        T* const out = dx + span.head + from * kE;
+        const Span os = span_of<DT>(out, places);
+        const uint32_t shift = os.head * (16 / kE);
+        uint4* const dv = reinterpret_cast<uint4*>(out + os.head);
+        const uint4* const xa = vec + from;  // vector i of dx is cut out of i and i + 1
+        for (uint32_t v0 = (threadIdx.x & ~31u) * 4; v0 < os.vecs; v0 += 4 * blockDim.x) {
+          uint4 q[4], last = make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int u = 0; u < 4; u++) {
+            const uint32_t v = v0 + u * 32 + lane;
+            q[u] = v < to - from ? load_with(xa + v, leave) : make_uint4(0, 0, 0, 0);
+          }
+          if (lane == 31 && v0 + 128 < to - from) last = load_with(xa + v0 + 128, leave);
 #pragma unroll
           for (int u = 0; u < 4; u++) {
             uint4 give = q[u];
@@ -560,31 +522,39 @@ __global__ void __launch_bounds__(kRowThreads<GRAD>, GRAD ? 2 : 5) distill_rows(
             uint4 next = make_uint4(__shfl_sync(0xffffffffu, give.x, lane + 1), __shfl_sync(0xffffffffu, give.y, lane + 1),
                                     __shfl_sync(0xffffffffu, give.z, lane + 1), __shfl_sync(0xffffffffu, give.w, lane + 1));
             if (u + 1 == 4 && lane == 31) next = last;
-            q[u] = shifted(q[u], next, shift);
+            const uint32_t v = v0 + u * 32 + lane;
+            if (v < os.vecs) __stcs(dv + v, tail_vec<DT>(shifted(q[u], next, shift), w, c2));
           }
-        } else {
-#pragma unroll
-          for (int u = 0; u < 4; u++)
-            if (v0 + u * 32 < os.vecs) q[u] = load_with(xa + v0 + u * 32, leave);
         }
-#pragma unroll
-        for (int u = 0; u < 4; u++)
-          if (v0 + u * 32 < os.vecs) __stcs(dv + v0 + u * 32, tail_vec<DT>(q[u], w, c2));
-      }
-      if (MOVED && threadIdx.x < 16) {
-        const uint32_t i = threadIdx.x & 7;
-        if (threadIdx.x < 8 ? i < os.head : i < os.tail) {
-          const uint32_t j = threadIdx.x < 8 ? i : os.head + os.vecs * kE + i;
-          out[j] = E::down(tail_of(E::up(x[span.head + from * kE + j]), w, c2));
+        if (threadIdx.x < 16) {
+          const uint32_t i = threadIdx.x & 7;
+          if (threadIdx.x < 8 ? i < os.head : i < os.tail) {
+            const uint32_t j = threadIdx.x < 8 ? i : os.head + os.vecs * kE + i;
+            out[j] = E::down(tail_of(E::up(x[span.head + from * kE + j]), w, c2));
+          }
         }
       }
-      if (edge_at != 0xffffffffu) dx[edge_at] = E::down(tail_of(edge, w, c2));
+      if (edge_at != 0xffffffffu) dx[edge_at] = E::down(tail_of(edges[threadIdx.x], w, c2));
+      __syncthreads();  // the list's places come last
+      if (mine) dx[entry.id] = E::down(ex2((xk - base_of(all.m)) * c2) * in_coef - weight * (float)entry.p);
     }
-    __syncthreads();  // the list's places come last; the bits are cleared
-    if constexpr (GRAD) {
-      if (mine) dx[now.id] = E::down(own);
+    if (a.loss.data && rank == 0 && threadIdx.x / 32 < list_warps) {
+      // sum P (log P - log q) with log q = scale (x - m) - log S; P > 0 at a masked place makes it infinite, P = 0 says nothing
+      const bool says = entry.p != 0.0 && entry.id != 0xffffffffu;
+      double2 dot = make_double2(says ? entry.p * ((double)a.scale * ((double)xk - (double)base_of(all.m))) : 0.0, 0.0);
+      dot = warp_sum(dot);
+      if (list_warps > 1) {
+        if ((threadIdx.x & 31) == 0) work.sums[threadIdx.x / 32] = dot;
+        list_sync(list_warps);
+        if (threadIdx.x < 32) dot = warp_sum(threadIdx.x < list_warps ? work.sums[threadIdx.x] : make_double2(0.0, 0.0));
+      }
+      if (threadIdx.x == 0) {
+        double loss = said.plogp - (dot.x - said.sum * (double)logf(all.s));
+        if (all.s == 0.0f) loss = said.sum > 0.0 ? (double)__int_as_float(0x7f800000) : 0.0;
+        if (tail > 0.0f) loss += (double)(tail * (logf(tail) - (logf(rest.s) + lead - logf(all.s))));
+        static_cast<float*>(a.loss.data)[row_at(a.g, a.loss, r)] = (float)loss;
+      }
     }
-    if (lists && r + stride < a.g.rows) mine = set_bits(r + stride);
     __syncthreads();
   }
   if (cluster > 1) cluster_wait();
@@ -604,13 +574,14 @@ cudaError_t launch_rows(const lc_context* ctx, const DistillArgs& a, uint32_t cl
   const uint64_t vecs = a.vocab / kE;
   const uint64_t share = std::max<uint64_t>(16, ((vecs + cluster - 1) / cluster + 15) / 16 * 16);
   const uint64_t busy = std::max<uint64_t>((share + kUnroll<DT> - 1) / kUnroll<DT>, a.list);
-  const uint32_t threads = (uint32_t)std::min<uint64_t>(kRowThreads<GRAD>, std::max<uint64_t>(32, (busy + 31) / 32 * 32));
+  // long slices: two blocks of 512 threads an SM, so that all rows under way stay in L2 for their second pass; shorter ones:
+  // four of 256, which leave each other less to wait for
+  const uint64_t most = share * 16 < kLongSlice ? 256 : kRowThreads<GRAD>;
+  const uint32_t threads = (uint32_t)std::min<uint64_t>(most, std::max<uint64_t>(32, (busy + 31) / 32 * 32));
   const bool moved = GRAD && apart(a.g, a.x, a.dx, 16 / kE);
   void (*kernel)(DistillArgs, uint32_t, uint32_t) = moved ? distill_rows<DT, GRAD, GRAD> : distill_rows<DT, GRAD, false>;
-  // with the gradient one wave of full blocks, which loop over the rows
-  const uint64_t most = GRAD && threads == kRowThreads<GRAD> && cluster == 1 ? 2 * ctx->sm_count : kMaxGrid;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(std::min<uint64_t>(a.g.rows, most) * cluster));
+  cfg.gridDim = dim3((unsigned)(std::min<uint64_t>(a.g.rows, kMaxGrid) * cluster));
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = share;
   cfg.stream = stream;

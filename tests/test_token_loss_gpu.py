@@ -493,6 +493,41 @@ def test_distill(ctx, dtype, n, v, k, tail):
     check_distill(ctx, x, ids, z, 0.5, tail, in_place=True)
 
 
+@pytest.mark.parametrize("dtype,v,k,pad,dpad", [("bf16", 16384, 16, 0, 0), ("bf16", 50001, 40, 63, 0), ("f16", 33003, 256, 0, 5),
+                                                ("f32", 40001, 64, 3, 0), ("f32", 8199, 1, 0, 0), ("bf16", 131075, 33, 5, 5)])
+def test_distill_many_rows(ctx, dtype, v, k, pad, dpad):
+    """More rows than the device takes at once, with lists of every length, masked rows among them, and rows of the logits
+    and of the gradient that start at different places within 16 bytes."""
+    n = 331
+    buf = torch.zeros(n, v + pad, device="cuda", dtype=TYPES[dtype])
+    x = buf[:, :v]
+    x.copy_(randn(n, v, seed=v) * 3 + randn(n, 1, seed=k) * 10)
+    x[5] = -INF
+    x[7, 100:] = -INF
+    x[9] = torch.finfo(TYPES[dtype]).min
+    ids, z = teacher_of(x, k, True)
+    ids[::3, k // 2:] = -1
+    ids[11] = -1
+    if k > 4:
+        ids[13, 2] = ids[13, 0]
+        ids[14, 0], ids[14, 1] = 0, v - 1
+        z[14, :2] = -3.0
+    d = randn(n, seed=4)
+    want_loss, tol_loss, want, tol = plain_distill(x, ids, z, 1.0, True, d)
+    out = torch.full((n, v + dpad), 5.0, device="cuda", dtype=TYPES[dtype])
+    loss = torch.empty(n, device="cuda")
+    for _ in range(2):
+        api.distill_grad(ctx, x, ids, z, 1.0, out[:, :v], d_loss=d, loss=loss, tail=True)
+        close(loss, want_loss, tol_loss, "loss")
+        close(out[:, :v], want, tol, "dlogits")
+        assert bool((out[:, v:] == 5).all())
+    first = out[:, :v].clone()
+    api.distill_grad(ctx, x, ids, z, 1.0, x, d_loss=d, tail=True)
+    close(x, want, tol, "in place")
+    if pad == dpad:
+        assert torch.equal(x, first)
+
+
 @pytest.mark.parametrize("tail", [False, True])
 @pytest.mark.parametrize("ttype", TYPES)
 def test_distill_padding_and_repeats(ctx, ttype, tail):
@@ -663,6 +698,44 @@ def test_streams_and_graphs(ctx):
     for i in range(2):
         assert all(torch.equal(a, b) for a, b in zip(flat(want[i]), flat(held[i][3])))
     assert all(torch.equal(a, b) for a, b in zip(flat(want[0]), flat(both[0])))
+
+
+def test_graphs_of_many_rows(ctx):
+    """Two captured calls over many rows, replayed at once, beside an eager one."""
+    n, v = 200, 20000
+    xs = [(randn(n, v, seed=i) * 3).bfloat16() for i in range(2)]
+    teach = [teacher_of(x, 16, True, seed=i) for i, x in enumerate(xs)]
+    want = []
+    for x, (ids, z) in zip(xs, teach):
+        dx, loss = torch.empty_like(x), torch.empty(n, device="cuda")
+        api.distill_grad(ctx, x, ids, z, 1.0, dx, loss=loss, tail=True)
+        want.append((dx, loss))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    graphs, held = [], []
+    for i in range(2):
+        x, ids, z = torch.zeros_like(xs[0]), torch.zeros_like(teach[0][0]), torch.zeros_like(teach[0][1])
+        dx, loss = torch.empty_like(x), torch.empty(n, device="cuda")
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=streams[i]):
+            lb.encode_distill_grad(ctx, streams[i], x, ids, z, 1.0, dx, loss=loss, tail=True)
+        graphs.append(g)
+        held.append((x, ids, z, dx, loss))
+    for i in range(2):
+        held[i][0].copy_(xs[i])
+        held[i][1].copy_(teach[i][0])
+        held[i][2].copy_(teach[i][1])
+    dx, loss = torch.empty_like(xs[0]), torch.empty(n, device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        lb.encode_distill_grad(ctx, None, xs[1], *teach[1], 1.0, dx, loss=loss, tail=True)
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(held[i][3], want[i][0]) and torch.equal(held[i][4], want[i][1])
+    assert torch.equal(dx, want[1][0]) and torch.equal(loss, want[1][1])
 
 
 def test_output_layer_step(ctx):

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -200,17 +201,41 @@ def check(code: int):
 # views over torch tensors
 # ---------------------------------------------------------------------------------------------
 
+_CODES: dict = {}
+
+
 def _dtype_code(t) -> int:
-    import torch
-    m = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.int32: I32,
-         torch.complex64: C32, torch.float64: F64, torch.complex128: C64}
-    if hasattr(torch, "uint32"):
-        m[torch.uint32] = U32
-    if hasattr(torch, "uint16"):
-        m[torch.uint16] = U16
-    if t.dtype not in m:
+    if not _CODES:
+        import torch
+        _CODES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.int32: I32,
+                       torch.complex64: C32, torch.float64: F64, torch.complex128: C64})
+        if hasattr(torch, "uint32"):
+            _CODES[torch.uint32] = U32
+        if hasattr(torch, "uint16"):
+            _CODES[torch.uint16] = U16
+    code = _CODES.get(t.dtype)
+    if code is None:
         raise TypeError(f"unsupported element type {t.dtype}")
-    return m[t.dtype]
+    return code
+
+
+_pack_view = struct.Struct("=QQQii8Q8Q").pack  # lc_view, filled in one go: a call makes a view of every operand
+_NO_AXES = [(0,) * (MAX_RANK - i) for i in range(MAX_RANK + 1)]
+
+
+def _view_of(t, dtype: int | None = None) -> lc_view:
+    st = t.untyped_storage()
+    code = _dtype_code(t) if dtype is None else dtype
+    shape, strides = t.shape, t.stride()
+    rank = len(shape)
+    if rank > MAX_RANK:
+        raise InvalidArgument(ERR_INVALID_ARGUMENT, "rank above 8")
+    none = _NO_AXES[rank]
+    try:
+        return lc_view.from_buffer_copy(_pack_view(st.data_ptr(), st.nbytes(), t.storage_offset(), code, rank, *shape, *none,
+                                                   *strides, *none))
+    except struct.error:
+        raise InvalidArgument(ERR_INVALID_ARGUMENT, "negative stride") from None
 
 
 class View:
@@ -225,21 +250,7 @@ class View:
 
     @staticmethod
     def of(t, dtype: int | None = None) -> "View":
-        st = t.untyped_storage()
-        v = lc_view()
-        v.data = st.data_ptr()
-        v.buffer_bytes = st.nbytes()
-        v.offset = t.storage_offset()
-        v.dtype = _dtype_code(t) if dtype is None else dtype
-        v.rank = t.dim()
-        if v.rank > MAX_RANK:
-            raise InvalidArgument(ERR_INVALID_ARGUMENT, "rank above 8")
-        for i, (n, s) in enumerate(zip(t.shape, t.stride())):
-            if s < 0:
-                raise InvalidArgument(ERR_INVALID_ARGUMENT, "negative stride")
-            v.shape[i] = n
-            v.strides[i] = s
-        return View(v, t)
+        return View(_view_of(t, dtype), t)
 
     @staticmethod
     def raw(owner, offset: int, shape, strides, dtype: int | None = None) -> "View":
@@ -325,8 +336,8 @@ def context() -> Context:
 
 
 def _stream(stream):
-    if stream is None:
-        return None
+    if stream is None or type(stream) is int:
+        return stream
     if hasattr(stream, "cuda_stream"):
         return stream.cuda_stream
     return stream
@@ -519,9 +530,11 @@ def relu_backward(ctx, pre, dy, dx, stream=None):
 # scores and losses over a vocabulary (no reference counterpart)
 # ---------------------------------------------------------------------------------------------
 
-def _maybe(x):
-    """A view by reference, or NULL for an operand that is not there."""
-    return None if x is None else as_view(x).ref()
+def _arg(x):
+    """An operand as the C calls take it: a view by reference, or NULL for one that is not there."""
+    if x is None:
+        return None
+    return x.c if isinstance(x, View) else _view_of(x)
 
 
 def encode_token_logprobs(ctx: Context, stream, logits, targets, scale=1.0, logprob=None, entropy=None, stats=None,
@@ -529,32 +542,32 @@ def encode_token_logprobs(ctx: Context, stream, logits, targets, scale=1.0, logp
     """Log probabilities of ``targets`` under softmax(scale * logits) over the last axis, with the rows' entropy,
     the ``stats`` that the gradient needs and the best alternatives; every output is optional, not all of them.
     A target outside [0, V), such as -1, stands for no token."""
-    check(load().lc_encode_token_logprobs(ctx.h, _stream(stream), as_view(logits).ref(), _maybe(targets), scale,
-                                          _maybe(logprob), _maybe(entropy), _maybe(stats), _maybe(top_logprobs),
-                                          _maybe(top_ids)))
+    check(load().lc_encode_token_logprobs(ctx.h, _stream(stream), _arg(logits), _arg(targets), scale,
+                                          _arg(logprob), _arg(entropy), _arg(stats), _arg(top_logprobs),
+                                          _arg(top_ids)))
 
 
 def encode_token_logprobs_backward(ctx: Context, stream, logits, targets, scale, stats, d_logprob, dlogits,
                                    entropy=None, d_entropy=None):
     """Gradient of ``encode_token_logprobs``' logprob and entropy; ``dlogits`` may be ``logits`` itself."""
-    check(load().lc_encode_token_logprobs_backward(ctx.h, _stream(stream), as_view(logits).ref(), _maybe(targets), scale,
-                                                   as_view(stats).ref(), _maybe(entropy), _maybe(d_logprob),
-                                                   _maybe(d_entropy), as_view(dlogits).ref()))
+    check(load().lc_encode_token_logprobs_backward(ctx.h, _stream(stream), _arg(logits), _arg(targets), scale,
+                                                   _arg(stats), _arg(entropy), _arg(d_logprob),
+                                                   _arg(d_entropy), _arg(dlogits)))
 
 
 def encode_distill_loss(ctx: Context, stream, logits, ids, teacher, scale, loss, tail=False):
     """Divergence of softmax(scale * logits) from a teacher's best alternatives (``ids``, ``teacher`` [..., K]):
     renormalised, or with ``tail`` as log probabilities whose rest is one bucket."""
-    check(load().lc_encode_distill_loss(ctx.h, _stream(stream), as_view(logits).ref(), as_view(ids).ref(),
-                                        as_view(teacher).ref(), scale, int(tail), as_view(loss).ref()))
+    check(load().lc_encode_distill_loss(ctx.h, _stream(stream), _arg(logits), _arg(ids),
+                                        _arg(teacher), scale, int(tail), _arg(loss)))
 
 
 def encode_distill_grad(ctx: Context, stream, logits, ids, teacher, scale, dlogits, d_loss=None, loss=None, tail=False):
     """``encode_distill_loss`` (``loss`` optional) and its gradient for ``d_loss`` (1 where None) in one pass;
     ``dlogits`` may be ``logits`` itself."""
-    check(load().lc_encode_distill_grad(ctx.h, _stream(stream), as_view(logits).ref(), as_view(ids).ref(),
-                                        as_view(teacher).ref(), scale, int(tail), _maybe(d_loss), _maybe(loss),
-                                        as_view(dlogits).ref()))
+    check(load().lc_encode_distill_grad(ctx.h, _stream(stream), _arg(logits), _arg(ids),
+                                        _arg(teacher), scale, int(tail), _arg(d_loss), _arg(loss),
+                                        _arg(dlogits)))
 
 
 def _waited(fn):

@@ -426,20 +426,20 @@ __global__ void __launch_bounds__(kRowThreads<GRAD>, kResident<DT, GRAD>) distil
         for (int u = 1; u < kU; u++) top = max_nan(top, Vec<DT>::top(q[u]));
         take<DT, kU, false>(run, q, top, c2);
       }
-      if (v0 < to) {
-        uint4 q[kU][1];
+      if (v0 + threadIdx.x < to) {  // the last step, short of some vectors: masked ones in their place
+        uint4 q[kU];
 #pragma unroll
         for (int u = 0; u < kU; u++) {
-          const uint32_t v = v0 + u * blockDim.x + threadIdx.x;
-          if (v < to) q[u][0] = GRAD ? load_with(vec + v, keep) : load_once(vec + v);
+          const uint4* p = vec + v0 + u * blockDim.x + threadIdx.x;
+          q[u] = v0 + u * blockDim.x + threadIdx.x >= to ? Vec<DT>::masked() : GRAD ? load_with(p, keep) : load_once(p);
         }
 #pragma unroll
-        for (int u = 0; u < kU; u++) {
-          const uint32_t v = v0 + u * blockDim.x + threadIdx.x;
-          if (v >= to) break;
-          take_out<DT>(q[u][0], bits[v]);
-          take<DT, 1, false>(run, q[u], Vec<DT>::top(q[u][0]), c2);
-        }
+        for (int u = 0; u < kU; u++)
+          if (v0 + u * blockDim.x + threadIdx.x < to) take_out<DT>(q[u], bits[v0 + u * blockDim.x + threadIdx.x]);
+        float top = Vec<DT>::top(q[0]);
+#pragma unroll
+        for (int u = 1; u < kU; u++) top = max_nan(top, Vec<DT>::top(q[u]));
+        take<DT, kU, false>(run, q, top, c2);
       }
     }
     Soft rest = soft_of(run, c2);

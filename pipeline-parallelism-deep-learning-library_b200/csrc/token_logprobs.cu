@@ -359,15 +359,6 @@ __global__ void __launch_bounds__(kMaxThreads, kResident<DT>) token_logprobs_row
     Run run = empty_run();
     uint32_t mine = 0, slot = 0, in_slot = 0;
     uint32_t* next = slots + threadIdx.x;
-    auto leave = [&](float top, bool last) {  // the largest of a step's logits goes to its slot
-      slot = max(slot, order_of(top));
-      if (++in_slot == per_slot || last) {
-        mine = max(mine, slot);
-        *next = slot;
-        next += blockDim.x;
-        slot = in_slot = 0;
-      }
-    };
     const uint32_t step = kSteps * blockDim.x;
     uint32_t v0 = sl.from;
     for (; v0 + step <= sl.to; v0 += step) {
@@ -378,30 +369,32 @@ __global__ void __launch_bounds__(kMaxThreads, kResident<DT>) token_logprobs_row
 #pragma unroll
       for (int u = 1; u < kSteps; u++) top = max_nan(top, Vec<DT>::top(q[u]));
       take<DT, kSteps, SUM_T>(run, q, top, c2);
-      if constexpr (TOP) leave(top, v0 + step >= sl.to);
+      if constexpr (TOP) {  // the largest of a step's logits goes to its slot
+        slot = max(slot, order_of(top));
+        if (++in_slot == per_slot || v0 + step >= sl.to) {
+          mine = max(mine, slot);
+          *next = slot;
+          next += blockDim.x;
+          slot = in_slot = 0;
+        }
+      }
     }
-    if (v0 < sl.to) {
-      uint4 q[kSteps][1];
+    if (v0 < sl.to) {  // the last step, short of some vectors: masked ones in their place
+      uint4 q[kSteps];
 #pragma unroll
       for (int u = 0; u < kSteps; u++) {
         const uint32_t v = v0 + u * blockDim.x + threadIdx.x;
-        if (v < sl.to) q[u][0] = load_once(sl.vec + v);
+        q[u] = v < sl.to ? load_once(sl.vec + v) : Vec<DT>::masked();
       }
-      float top = neg_inf();
+      const bool any = v0 + threadIdx.x < sl.to;
+      float top = Vec<DT>::top(q[0]);
 #pragma unroll
-      for (int u = 0; u < kSteps; u++) {
-        if (v0 + u * blockDim.x + threadIdx.x >= sl.to) break;
-        const float t = Vec<DT>::top(q[u][0]);
-        top = max_nan(top, t);
-        take<DT, 1, SUM_T>(run, q[u], t, c2);
-      }
+      for (int u = 1; u < kSteps; u++) top = max_nan(top, Vec<DT>::top(q[u]));
+      if (any) take<DT, kSteps, SUM_T>(run, q, top, c2);
       if constexpr (TOP) {
-        if (v0 + threadIdx.x < sl.to) {
-          leave(top, true);
-        } else {  // nothing of this step is this thread's
-          mine = max(mine, slot);
-          *next = slot;
-        }
+        if (any) slot = max(slot, order_of(top));
+        mine = max(mine, slot);
+        *next = slot;
       }
     }
     Soft part = soft_of(run, c2);
@@ -427,8 +420,8 @@ __global__ void __launch_bounds__(kMaxThreads, kResident<DT>) token_logprobs_row
     }
     if (rank == 0) {
       if (cluster > 1) {
-        row = parts[0];
-        for (uint32_t c = 1; c < cluster; c++) row = merge(row, parts[c], c2);
+        const uint32_t c = threadIdx.x & 31;
+        row = warp_merge(c < cluster ? parts[c] : Soft{neg_inf(), 0.0f, 0.0f}, c2);
       }
       const float total = logf(row.s);
       if (threadIdx.x == 0) write_row(a, r, row, total, token, xt);
@@ -436,20 +429,13 @@ __global__ void __launch_bounds__(kMaxThreads, kResident<DT>) token_logprobs_row
         if (cluster == 1) {
           for (uint32_t k = threadIdx.x; k < a.top; k += blockDim.x) write_best(a, r, k, best[k], row, total);
         } else {
-          // the K best of the blocks' lists, each of them in order: a key's rank is how many are better in every list
-          for (uint32_t i = threadIdx.x; i < cluster * a.top; i += blockDim.x) {
+          // the K best of the blocks' lists, told apart by rank
+          const uint32_t n = cluster * a.top;
+          for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
             const uint64_t key = lists[i];
             uint32_t k = key ? 0 : a.top;
-            for (uint32_t c = 0; c < cluster && k < a.top; c++) {
-              const uint64_t* list = lists + c * a.top;
-              uint32_t lo = 0, hi = a.top;
-              while (lo < hi) {
-                const uint32_t mid = (lo + hi) / 2;
-                if (list[mid] > key) lo = mid + 1;
-                else hi = mid;
-              }
-              k += lo;
-            }
+#pragma unroll 8
+            for (uint32_t o = 0; o < n; o++) k += lists[o] > key;
             if (k < a.top) write_best(a, r, k, key, row, total);
           }
         }

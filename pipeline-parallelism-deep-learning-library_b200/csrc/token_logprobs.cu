@@ -103,7 +103,7 @@ constexpr int kMaxThreads = 256;
 template <int DT>
 constexpr int kUnroll = 32 / Vec<DT>::kElems;  // vectors of a step: 32 places a thread
 template <int DT>
-constexpr int kResident = DT == LC_F32 ? 5 : 6;  // blocks an SM
+constexpr int kResident = DT == LC_F32 ? 4 : 6;  // blocks an SM
 constexpr uint32_t kMaxSlots = 4096;
 constexpr uint32_t kMaxKeys = 512;
 constexpr uint32_t kMaxRead = 256;  // slots that are read again in one go
@@ -654,7 +654,7 @@ Spread spread_of(const lc_context* ctx, uint64_t rows, uint64_t vocab, uint32_t 
   Spread s{};
   const uint64_t vecs = vocab / elems;
   s.cluster = 1;
-  while (s.cluster < kMaxCluster && rows * s.cluster < 2ull * ctx->sm_count && vecs / (2 * s.cluster) >= 2ull * unroll * 256)
+  while (s.cluster < kMaxCluster && rows * s.cluster < 2ull * ctx->sm_count && vecs / (2 * s.cluster) >= 1ull * unroll * 256)
     s.cluster *= 2;
   const uint64_t share = std::max<uint64_t>(((vecs + s.cluster - 1) / s.cluster + 31) / 32 * 32, 1);
   const uint64_t busy = std::max<uint64_t>((share + unroll - 1) / unroll, 2 * top);

@@ -207,13 +207,23 @@ __global__ void __launch_bounds__(kThreads) distill_strided(DistillArgs a) {
 //
 // One block a row, or a cluster of blocks where there are few rows, each with a slice.  Two passes over the slice: the sums,
 // in which a bit for each place tells the list's places, and the gradient.  Between them the blocks of a cluster tell one
-// another their sums.  The second pass finds the row in L2, so it crosses HBM once each way.
+// another their sums.  The second pass finds most of the row in L2: the first reads it with a policy that keeps it there,
+// the second one that lets it go, and the gradient is stored past the caches.
+//
+// What bounds it (B200, of the 6465 GB/s of a copy).  The loss alone reads HBM at 6117 GB/s (4096 x 131,072 bf16, 64 entries:
+// 176 us).  With the gradient it is 454 us, 4737 GB/s of the bytes that must move: 1.16 times the logits come from HBM
+// (some lines are gone before the second pass), and a block's chain from its list over the sums to the gradient leaves the
+// memory idle where the other block of its SM cannot fill in.  Tried and slower: the row in shared memory over a cluster of
+// 8 blocks filled by the copy engine, one pass after the other (755 us) or with the next row's sums before this row's
+// gradient (811 us; the fixed work of a block weighs 8 times); the first 88 KB of a row in shared memory (527 us); lists a
+// row ahead and gradient tiles to whichever warp is free (486 us); three or four smaller blocks an SM (505 to 521 us: more
+// rows under way than L2 holds).
 template <int DT>
 constexpr int kUnroll = 32 / Vec<DT>::kElems;  // vectors of a step: 32 places a thread
 template <bool GRAD>
 constexpr int kRowThreads = GRAD ? 512 : 256;
 template <int DT, bool GRAD>
-constexpr int kResident = GRAD ? 2 : DT == LC_F32 ? 4 : 6;  // blocks an SM
+constexpr int kResident = GRAD ? 2 : DT == LC_F32 ? 4 : 6;  // blocks an SM (loss alone, bf16: 178 us with 6, 197 with 4)
 constexpr uint32_t kMaxCluster = 8;
 constexpr uint64_t kLongSlice = 128 << 10;  // bytes
 constexpr uint64_t kMaxBits = 64 << 10;  // bytes of shared memory for a slice's bits
@@ -345,14 +355,13 @@ __device__ __forceinline__ void take_out(uint4& q, uint32_t bits) {
   q = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// A place's byte and bit: a byte a vector (of f32 four bits are used).
 template <int DT, bool GRAD, bool MOVED>
 __global__ void __launch_bounds__(kRowThreads<GRAD>, kResident<DT, GRAD>) distill_rows(DistillArgs a, uint32_t cluster, uint32_t share) {
   using E = Elem<DT>;
   using T = typename E::T;
   constexpr uint32_t kE = Vec<DT>::kElems;
   constexpr int kU = kUnroll<DT>;
-  extern __shared__ __align__(16) uint8_t in_list[];  // [share], a multiple of 16
+  extern __shared__ __align__(16) uint8_t in_list[];  // [share], a multiple of 16: a byte a vector, a bit a place
   __shared__ uint32_t ids[kMaxList];
   __shared__ Soft red[kRowThreads<GRAD> / 32];
   __shared__ float edges[16];
@@ -574,8 +583,8 @@ cudaError_t launch_rows(const lc_context* ctx, const DistillArgs& a, uint32_t cl
   const uint64_t vecs = a.vocab / kE;
   const uint64_t share = std::max<uint64_t>(16, ((vecs + cluster - 1) / cluster + 15) / 16 * 16);
   const uint64_t busy = std::max<uint64_t>((share + kUnroll<DT> - 1) / kUnroll<DT>, a.list);
-  // long slices: two blocks of 512 threads an SM, so that all rows under way stay in L2 for their second pass; shorter ones:
-  // four of 256, which leave each other less to wait for
+  // long slices: two blocks of 512 threads an SM, so that most of the rows under way stay in L2 for their second pass (4096 x
+  // 131,072 bf16: 463 us, 505 with four of 256); shorter ones: four of 256 (777 x 50,001 bf16: 54.6 us, 59.5 with two of 512)
   const uint64_t most = share * 16 < kLongSlice ? 256 : kRowThreads<GRAD>;
   const uint32_t threads = (uint32_t)std::min<uint64_t>(most, std::max<uint64_t>(32, (busy + 31) / 32 * 32));
   const bool moved = GRAD && apart(a.g, a.x, a.dx, 16 / kE);

@@ -92,18 +92,30 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_strided(ScoreArgs a) 
 
 // ---- the vocabulary as the unit axis -----------------------------------------------------------
 //
-// One cluster of blocks a row (one block where there are rows enough): each thread takes up 4 vectors of 16 bytes at a time
-// into its own running softmax; threads, blocks and the cluster merge them once at the end, in an order that does not vary.
+// One cluster of blocks a row (one block where there are rows enough): each thread takes up 32 places at a time into its own
+// running softmax; threads, blocks and the cluster merge them once at the end, in an order that does not vary.
 //
-// The alternatives come out of the same pass.  Each thread leaves the order of the largest logit of every 4 vectors (a
-// slot) in shared memory.  A bound that at least K places reach is known without looking at a place again: of the threads'
-// own largest, the q-th best of each warp, q = K over the number of warps, and of those the least.  Only slots above the
-// bound are read again (some 70 of 4096 for K = 20 of 131,072), and what lies above it is ranked by counting.
+// The alternatives come out of the same pass.  Each thread leaves the order of the largest logit of every step (a slot) in
+// shared memory.  A bound that at least K places reach is known without looking at a place again: of the threads' own
+// largest, the q-th best of each warp, q = K over the number of warps, and of those the least.  Only slots above the bound
+// are read again (some 80 of 4096 for K = 20 of 131,072), and what lies above it is ranked by counting.  Rows whose best
+// places crowd together beyond what shared memory holds (a narrow band, a few thousand permitted places side by side) find
+// the K-th largest order bit by bit instead: right for every row, and slower.
+//
+// What bounds it (B200, whole call in a graph, of the 6465 GB/s of a copy): HBM.  2048 x 100,003 f32 with entropy reads at
+// 6448 GB/s (127 us), 4096 x 131,072 bf16 at 6256 (172 us); f16 and bf16 have two exponentials for each of f32 and three
+// quarters of the exponential unit's rate at that speed.  The alternatives cost 26 us more with K = 20 (198 us; 208 with the
+// entropy too): a block waits for one more read from L2 and some barriers, which the other blocks of its SM cover in part.
+// Why small blocks and not a ring of stages that the copy engine fills (3 of 32 KB a block, two blocks of 512 an SM,
+// measured: 224 us against 182 with four blocks of 256 and plain loads, 173 with six): a block's end is a chain of barriers,
+// and only other blocks can fill it.
+// A single row (1 x 131,072 bf16, K = 20) takes 9.8 us over a cluster of 8, nearly all of it latency: 1.4 us to the logits,
+// 0.7 to merge, 3.6 for the block's alternatives, the rest for the cluster's.  16 blocks a cluster measured 13.5 us.
 constexpr int kMaxThreads = 256;
 template <int DT>
 constexpr int kUnroll = 32 / Vec<DT>::kElems;  // vectors of a step: 32 places a thread
 template <int DT>
-constexpr int kResident = DT == LC_F32 ? 4 : 6;  // blocks an SM
+constexpr int kResident = DT == LC_F32 ? 4 : 6;  // blocks an SM; 16-bit types: 173 us with 6, 183 with 4 (4096 x 131,072)
 constexpr uint32_t kMaxSlots = 4096;
 constexpr uint32_t kMaxKeys = 512;
 constexpr uint32_t kMaxRead = 256;  // slots that are read again in one go
@@ -557,6 +569,10 @@ __device__ __forceinline__ uint4 grad_vec(const uint4& q, uint32_t j, const Grad
 // padded rows).  A vector of it then is cut out of two aligned ones, of which the second comes from the next lane (a
 // warp's vectors of a step follow one another), or at the end of a warp's vectors from a load of its own.  In steps that reach the row's ends the vectors are read one by one, as
 // are the places around them.
+// Bound by HBM: 4096 x 131,072 bf16 with the entropy's share 331 us, 6495 GB/s, as fast as a copy; stores that stream past
+// the caches and four blocks an SM with registers enough for all loads of a step (434 us with six and spills).  MOVED rows
+// (1001 x 50,001 bf16 in padded rows: 43 us, 4650 GB/s; 37 us were the rows alike) pay for the shifts, which keep the ALU
+// busy; two loads a vector instead of the neighbour's half measured 53 us.
 constexpr int kGradUnroll = 4;
 
 template <int DT, bool ENT, bool MOVED>
@@ -647,9 +663,10 @@ struct Spread {
   size_t shared;
 };
 
-// Enough blocks to fill the device, as long as each has 2 steps of 512 threads left to do: one row of 131,072 bf16 over 8
-// blocks.  From 2 rows an SM on, one block a row.  A block has the threads that its vectors keep busy at 4 each, and 2 for
-// each alternative asked for, so that the bound on them (select) comes from several warps.
+// Enough blocks to fill the device, as long as each has a step of 256 threads left to do: one row of 131,072 bf16 over 8
+// blocks (37 x 50,001 f32: 9.8 us over 8 blocks a row, 11.2 over 4).  From 2 rows an SM on, one block a row: clusters of 2
+// for 2048 rows measured 86 us against 77.  A block has the threads that its vectors keep busy, and 2 for each alternative
+// asked for, so that the bound on them (select) comes from several warps.
 Spread spread_of(const lc_context* ctx, uint64_t rows, uint64_t vocab, uint32_t elems, uint32_t unroll, uint32_t top) {
   Spread s{};
   const uint64_t vecs = vocab / elems;

@@ -316,14 +316,6 @@ __device__ __forceinline__ float logprob_of(float x, float m, float total, float
   return x == neg_inf() && !isnan(m) && !isnan(total) ? neg_inf() : __fsub_rn(__fmul_rn(__fsub_rn(x, m), scale), total);
 }
 
-// Copies `bytes` (a multiple of 16, both ends on 16-byte boundaries) into shared memory; they count on `bar`.
-__device__ __forceinline__ void copy_in(void* to, const void* from, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   (uint32_t)__cvta_generic_to_shared(to)),
-               "l"(from), "r"(bytes), "r"((uint32_t)__cvta_generic_to_shared(bar))
-               : "memory");
-}
-
 // ---- a row shared by the blocks of a cluster --------------------------------------------------
 
 // The 16-byte vectors of a row: `head` places before the first aligned one, `vecs` whole ones, `tail` places behind them.

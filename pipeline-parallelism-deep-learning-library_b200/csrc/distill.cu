@@ -210,10 +210,11 @@ __global__ void __launch_bounds__(kThreads) distill_strided(DistillArgs a) {
 // another their sums.  The second pass finds most of the row in L2: the first reads it with a policy that keeps it there,
 // the second one that lets it go, and the gradient is stored past the caches.
 //
-// What bounds it (B200, of the 6465 GB/s of a copy).  The loss alone reads HBM at 6117 GB/s (4096 x 131,072 bf16, 64 entries:
-// 176 us).  With the gradient it is 454 us, 4737 GB/s of the bytes that must move: 1.16 times the logits come from HBM
+// What bounds it (B200, of the 6465 GB/s of a copy).  The loss alone reads HBM at 6128 GB/s (4096 x 131,072 bf16, 64 entries:
+// 176 us).  With the gradient it is 446 us, 4818 GB/s of the bytes that must move: 1.16 times the logits come from HBM
 // (some lines are gone before the second pass), and a block's chain from its list over the sums to the gradient leaves the
-// memory idle where the other block of its SM cannot fill in.  Tried and slower: the row in shared memory over a cluster of
+// memory idle where the other block of its SM cannot fill in.  A fetch of the row's first half into L2 before the list took
+// 454 to 446 us (4096 x 32,768 f32: 203 to 192); of the whole row, 509; on short rows and for the loss alone it cost time.  Tried and slower: the row in shared memory over a cluster of
 // 8 blocks filled by the copy engine, one pass after the other (755 us) or with the next row's sums before this row's
 // gradient (811 us; the fixed work of a block weighs 8 times); the first 88 KB of a row in shared memory (527 us); lists a
 // row ahead and gradient tiles to whichever warp is free (486 us); three or four smaller blocks an SM (505 to 521 us: more
@@ -226,6 +227,7 @@ template <int DT, bool GRAD>
 constexpr int kResident = GRAD ? 2 : DT == LC_F32 ? 4 : 6;  // blocks an SM (loss alone, bf16: 178 us with 6, 197 with 4)
 constexpr uint32_t kMaxCluster = 8;
 constexpr uint64_t kLongSlice = 128 << 10;  // bytes
+constexpr uint32_t kAhead = 8192;  // vectors
 constexpr uint64_t kMaxBits = 64 << 10;  // bytes of shared memory for a slice's bits
 
 // A thread's entry of the list.
@@ -378,6 +380,9 @@ __global__ void __launch_bounds__(kRowThreads<GRAD>, kResident<DT, GRAD>) distil
     const Span span = span_of<DT>(x, a.vocab);
     const uint32_t from = min(span.vecs, rank * share), to = min(span.vecs, from + share);
     const uint4* vec = reinterpret_cast<const uint4*>(x + span.head);
+    // the first 128 KB of a long slice come while the list does, a line of 8 vectors at a time
+    if (GRAD && blockDim.x == kRowThreads<GRAD>)
+      for (uint32_t v = from + threadIdx.x * 8; v < min(to, from + kAhead); v += blockDim.x * 8) bring_to_l2(vec + v);
     Entry entry{0xffffffffu, 0.0};
     float z = neg_inf(), xk = neg_inf();
     if (threadIdx.x < a.list) {

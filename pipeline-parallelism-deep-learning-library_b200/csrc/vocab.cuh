@@ -164,6 +164,7 @@ __device__ __forceinline__ uint64_t leave_l2() {
   asm volatile("createpolicy.fractional.L2::evict_first.b64 %0;" : "=l"(p));
   return p;
 }
+__device__ __forceinline__ void bring_to_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 __device__ __forceinline__ uint4 load_with(const void* p, uint64_t policy) {
   uint4 q;
   asm volatile("ld.global.L1::no_allocate.L2::cache_hint.v4.u32 {%0, %1, %2, %3}, [%4], %5;"

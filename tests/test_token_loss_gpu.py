@@ -140,7 +140,7 @@ def test_scores(ctx, dtype, n, v, k):
     check_scores(ctx, x, tokens(n, v), 1.0, k)
 
 
-@pytest.mark.parametrize("scale", [1e-3, 0.7, 1.0, 3.0, 200.0])
+@pytest.mark.parametrize("scale", [1e-6, 1e-3, 0.7, 1.0, 3.0, 200.0, 1e5])
 def test_scores_scale(ctx, scale):
     x = randn(6, 5003, seed=2) * 4
     check_scores(ctx, x, tokens(6, 5003), scale, 7)

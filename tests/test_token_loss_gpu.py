@@ -140,6 +140,14 @@ def test_scores(ctx, dtype, n, v, k):
     check_scores(ctx, x, tokens(n, v), 1.0, k)
 
 
+@pytest.mark.parametrize("dtype,n,v,k", [("bf16", 301, 150001, 20), ("f32", 300, 140003, 64), ("f16", 1, 4300001, 128)])
+def test_scores_long(ctx, dtype, n, v, k):
+    """Rows so long that several steps of a block share what it notes for the alternatives."""
+    x = (randn(n, v, seed=3) * 3).to(TYPES[dtype])
+    x[0, : v - 4000] = -INF  # the best places side by side
+    check_scores(ctx, x, tokens(n, v), 1.0, k)
+
+
 @pytest.mark.parametrize("scale", [1e-6, 1e-3, 0.7, 1.0, 3.0, 200.0, 1e5])
 def test_scores_scale(ctx, scale):
     x = randn(6, 5003, seed=2) * 4
@@ -526,6 +534,14 @@ def test_distill_many_rows(ctx, dtype, v, k, pad, dpad):
     close(x, want, tol, "in place")
     if pad == dpad:
         assert torch.equal(x, first)
+
+
+@pytest.mark.parametrize("tail", [False, True])
+def test_distill_longest(ctx, tail):
+    """A vocabulary whose places' bits do not fit in a cluster's shared memory."""
+    x = (randn(2, 4300001, seed=3) * 3).bfloat16()
+    ids, z = teacher_of(x, 40, tail)
+    check_distill(ctx, x, ids, z, 1.0, tail, d_loss=randn(2, seed=4))
 
 
 @pytest.mark.parametrize("tail", [False, True])

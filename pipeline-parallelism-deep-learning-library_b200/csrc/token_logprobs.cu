@@ -224,7 +224,7 @@ __device__ void select(const Slice& sl, const uint32_t* slots, uint32_t mine, ui
   const uint32_t reads = count[1], per = sl.per_slot * kSteps;
   if (reads <= kMaxRead) {
     for (uint32_t i = threadIdx.x; i < reads * per; i += blockDim.x) {
-      const uint32_t e = w.read[i / per], k = i % per;
+      const uint32_t slot = sl.per_slot == 1 ? i / kSteps : i / per, e = w.read[slot], k = i - slot * per;
       const uint32_t v = sl.from + ((e >> 16) * per + k) * blockDim.x + (e & 0xffffu);
       if (v >= sl.to) continue;
       const uint4 q = __ldg(sl.vec + v);

@@ -304,7 +304,8 @@ lc_status lc_encode_token_logprobs_backward(lc_context* ctx, void* stream, const
  *   tail 1: teacher holds log probabilities, P = e^teacher; what they leave, r = max(0, 1 - sum P),
  *           is one bucket against the student's Q outside the list:
  *           loss = sum P (log P - log q_id) + r (log r - log Q), the bucket left out where Q = 0
- * A row without entries has loss 0 (tail 0: and no gradient). */
+ * A row without entries has loss 0 (tail 0: and no gradient).  P above 0 at a masked place makes the
+ * loss infinite; the gradient there is -P all the same. */
 lc_status lc_encode_distill_loss(lc_context* ctx, void* stream, const lc_view* logits,
                                  const lc_view* ids, const lc_view* teacher, float scale, int32_t tail,
                                  const lc_view* loss);

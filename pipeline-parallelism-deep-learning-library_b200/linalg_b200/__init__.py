@@ -530,11 +530,16 @@ def relu_backward(ctx, pre, dy, dx, stream=None):
 # scores and losses over a vocabulary (no reference counterpart)
 # ---------------------------------------------------------------------------------------------
 
-def _arg(x):
-    """An operand as the C calls take it: a view by reference, or NULL for one that is not there."""
+def _arg(ctx: Context, x):
+    """An operand as the C calls take it: a view by reference, or NULL for one that is not there.  A tensor has to
+    lie on the context's device; a kernel that followed the address of any other would fault."""
     if x is None:
         return None
-    return x.c if isinstance(x, View) else _view_of(x)
+    if isinstance(x, View):
+        return x.c
+    if x.get_device() != ctx.device:
+        raise InvalidArgument(ERR_INVALID_ARGUMENT, f"operand on {x.device}, not on the context's device cuda:{ctx.device}")
+    return _view_of(x)
 
 
 def encode_token_logprobs(ctx: Context, stream, logits, targets, scale=1.0, logprob=None, entropy=None, stats=None,
@@ -542,32 +547,32 @@ def encode_token_logprobs(ctx: Context, stream, logits, targets, scale=1.0, logp
     """Log probabilities of ``targets`` under softmax(scale * logits) over the last axis, with the rows' entropy,
     the ``stats`` that the gradient needs and the best alternatives; every output is optional, not all of them.
     A target outside [0, V), such as -1, stands for no token."""
-    check(load().lc_encode_token_logprobs(ctx.h, _stream(stream), _arg(logits), _arg(targets), scale,
-                                          _arg(logprob), _arg(entropy), _arg(stats), _arg(top_logprobs),
-                                          _arg(top_ids)))
+    check(load().lc_encode_token_logprobs(ctx.h, _stream(stream), _arg(ctx, logits), _arg(ctx, targets), scale,
+                                          _arg(ctx, logprob), _arg(ctx, entropy), _arg(ctx, stats), _arg(ctx, top_logprobs),
+                                          _arg(ctx, top_ids)))
 
 
 def encode_token_logprobs_backward(ctx: Context, stream, logits, targets, scale, stats, d_logprob, dlogits,
                                    entropy=None, d_entropy=None):
     """Gradient of ``encode_token_logprobs``' logprob and entropy; ``dlogits`` may be ``logits`` itself."""
-    check(load().lc_encode_token_logprobs_backward(ctx.h, _stream(stream), _arg(logits), _arg(targets), scale,
-                                                   _arg(stats), _arg(entropy), _arg(d_logprob),
-                                                   _arg(d_entropy), _arg(dlogits)))
+    check(load().lc_encode_token_logprobs_backward(ctx.h, _stream(stream), _arg(ctx, logits), _arg(ctx, targets), scale,
+                                                   _arg(ctx, stats), _arg(ctx, entropy), _arg(ctx, d_logprob),
+                                                   _arg(ctx, d_entropy), _arg(ctx, dlogits)))
 
 
 def encode_distill_loss(ctx: Context, stream, logits, ids, teacher, scale, loss, tail=False):
     """Divergence of softmax(scale * logits) from a teacher's best alternatives (``ids``, ``teacher`` [..., K]):
     renormalised, or with ``tail`` as log probabilities whose rest is one bucket."""
-    check(load().lc_encode_distill_loss(ctx.h, _stream(stream), _arg(logits), _arg(ids),
-                                        _arg(teacher), scale, int(tail), _arg(loss)))
+    check(load().lc_encode_distill_loss(ctx.h, _stream(stream), _arg(ctx, logits), _arg(ctx, ids),
+                                        _arg(ctx, teacher), scale, int(tail), _arg(ctx, loss)))
 
 
 def encode_distill_grad(ctx: Context, stream, logits, ids, teacher, scale, dlogits, d_loss=None, loss=None, tail=False):
     """``encode_distill_loss`` (``loss`` optional) and its gradient for ``d_loss`` (1 where None) in one pass;
     ``dlogits`` may be ``logits`` itself."""
-    check(load().lc_encode_distill_grad(ctx.h, _stream(stream), _arg(logits), _arg(ids),
-                                        _arg(teacher), scale, int(tail), _arg(d_loss), _arg(loss),
-                                        _arg(dlogits)))
+    check(load().lc_encode_distill_grad(ctx.h, _stream(stream), _arg(ctx, logits), _arg(ctx, ids),
+                                        _arg(ctx, teacher), scale, int(tail), _arg(ctx, d_loss), _arg(ctx, loss),
+                                        _arg(ctx, dlogits)))
 
 
 def _waited(fn):

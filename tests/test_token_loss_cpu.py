@@ -187,3 +187,20 @@ def test_distill_outputs():
 @pytest.mark.parametrize("call", CALLS)
 def test_no_rows_still_checked(call):
     refused(call(logits=view([0, V], lb.BF16)), "leading shape")
+
+
+def test_tensors_elsewhere():
+    """A tensor that does not lie on the context's device never reaches the library."""
+    import torch
+
+    class Ctx:
+        h, device = None, 0
+
+    x, t = torch.zeros(N, V), torch.zeros(N, dtype=torch.int32)
+    n, n2, nk, ids = torch.zeros(N), torch.zeros(N, 2), torch.zeros(N, K), torch.zeros(N, K, dtype=torch.int32)
+    for call in (lambda: lb.encode_token_logprobs(Ctx, None, x, t, 1.0, logprob=n),
+                 lambda: lb.encode_token_logprobs_backward(Ctx, None, x, t, 1.0, n2, n, x),
+                 lambda: lb.encode_distill_loss(Ctx, None, x, ids, nk, 1.0, n),
+                 lambda: lb.encode_distill_grad(Ctx, None, x, ids, nk, 1.0, x)):
+        with pytest.raises(lb.InvalidArgument, match="not on the context's device"):
+            call()

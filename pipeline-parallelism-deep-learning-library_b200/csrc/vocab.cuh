@@ -226,18 +226,20 @@ __device__ __forceinline__ Soft block_merge(Soft v, float c2, Soft* red) {
 
 // The softmax of what one thread has seen, in two lanes of sums.
 //
-// While the largest logit is of an ordinary size, d is one fused multiply-add, x c2 - mc, against mc = m c2 as it rounds:
-// one rounding a place, as good as (x - m) c2 with its two.  The sums then stand against mc / c2 and not m; soft_of moves
-// them by the difference.  Logits beyond kWide, where x c2 could overflow or places could not be told from masked ones, and
-// scales far from 1 take (x - m) c2.
+// While m c2 is of an ordinary size, d is one fused multiply-add, x c2 - mc, against mc = m c2 as it rounds: one rounding a
+// place, as good as (x - m) c2 with its two.  The sums then stand against mc / c2 and not m; soft_of moves them by the
+// difference, off = m c2 - mc.  2^off is a factor of every sum on the way, and off is up to half a step of mc: it stays within
+// 2^-5 below kWide, and would overflow the sums from 2^31 on (logits of -1e10, as forbidden tokens are often filled with).
+// Rows beyond kWide, and scales far from 1, take (x - m) c2.  What a thread has seen may pass the border either way (its
+// first places forbidden, say): the sums then move by the exact distance between what they stood against and what they will.
 struct Run {
   float m, mc;
   float2 s, t;
 };
-constexpr float kWide = 1e25f;
+constexpr float kWide = 1048576.0f;
 __device__ __forceinline__ Run empty_run() { return Run{neg_inf(), 0.0f, make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)}; }
 // NaN and the infinities are wide
-__device__ __forceinline__ bool is_wide(float m, float c2) { return !(fabsf(m) < kWide) || !(c2 > 1e-3f && c2 < 1e4f); }
+__device__ __forceinline__ bool is_wide(float m, float c2) { return !(fabsf(m * c2) < kWide) || !(c2 > 1e-3f && c2 < 1e4f); }
 
 // Takes up N vectors whose largest logit is `top`.  SUM_T: with the sum that the entropy needs.
 template <int DT, int N, bool SUM_T>
@@ -246,7 +248,8 @@ __device__ __forceinline__ void take(Run& r, const uint4 (&q)[N], float top, flo
   const bool wide = is_wide(m, c2);
   if (!(m == r.m)) {  // a new largest logit (or a NaN): seldom, after the first vectors of a row
     const float mc = wide ? 0.0f : m * c2;
-    float u = wide || is_wide(r.m, c2) ? (r.m - base_of(m)) * c2 : r.mc - mc;
+    const bool was = is_wide(r.m, c2);
+    float u = wide ? (was ? (r.m - base_of(m)) * c2 : -__fmaf_rn(m, c2, -r.mc)) : was ? __fmaf_rn(r.m, c2, -mc) : r.mc - mc;
     u = r.m == neg_inf() ? 0.0f : max_nan(u, kFar);
     const float2 f = both(ex2(u));
     if constexpr (SUM_T) r.t = __fmul2_rn(f, __ffma2_rn(both(u), r.s, r.t));
@@ -279,7 +282,7 @@ __device__ __forceinline__ void take(Run& r, const uint4 (&q)[N], float top, flo
   const float2 minus = both(-base_of(r.m));
 #pragma unroll
   for (int n = 0; n < N; n++)
-#pragma unroll 1
+#pragma unroll
     for (int i = 0; i < Vec<DT>::kElems / 2; i++) {
       const float2 d = __fmul2_rn(__fadd2_rn(Vec<DT>::pair(q[n], i), minus), c);
       const float2 e = make_float2(ex2(d.x), ex2(d.y));

@@ -606,7 +606,9 @@ cudaError_t launch_rows(const lc_context* ctx, const DistillArgs& a, uint32_t cl
   cfg.attrs = at;
   cfg.numAttrs = cluster > 1 ? 1 : 0;
   if (cfg.dynamicSmemBytes > (40 << 10)) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes);
+    // the bound belongs to the kernel on its device and not to the call: always the most that any call needs, so that no thread
+    // lowers another's between its setting and its launch
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxBits);
     if (e != cudaSuccess) return e;
   }
   return cudaLaunchKernelEx(&cfg, kernel, a, cluster, (uint32_t)share);

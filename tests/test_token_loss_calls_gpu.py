@@ -1,0 +1,50 @@
+"""How the operators over a vocabulary are called: from threads, on streams, and what the context says of it."""
+import threading
+
+import pytest
+import torch
+
+import linalg_b200 as lb
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx(gpu):
+    return lb.Context(0)
+
+
+def test_long_rows_from_threads(ctx):
+    """Vocabularies whose kernel takes more shared memory than any kernel may without asking, of several sizes, from threads
+    at once: no call takes from another what it asked for."""
+    jobs = []
+    for v in (2_000_000, 1_400_000, 1_900_000, 1_500_000):
+        x = torch.randn(1, v, device="cuda", generator=torch.Generator("cuda").manual_seed(v))
+        ids, z = torch.arange(4, device="cuda").int()[None], torch.full((1, 4), -2.0, device="cuda")
+        loss = torch.empty(1, device="cuda")
+        jobs.append([lb.View.of(t) for t in (x, ids, z, loss)] + [torch.cuda.Stream().cuda_stream])
+    torch.cuda.synchronize()
+    want, failed = [], []
+    for x, ids, z, loss, _ in jobs:
+        lb.distill_loss(ctx, x, ids, z, 1.0, loss, tail=True)
+        want.append(loss.owner.clone())
+    torch.cuda.synchronize()
+    start = threading.Barrier(len(jobs))
+
+    def work(x, ids, z, loss, stream):
+        start.wait()
+        try:
+            for _ in range(4000):
+                lb.encode_distill_loss(ctx, stream, x, ids, z, 1.0, loss, tail=True)
+        except lb.LinalgError as e:
+            failed.append(str(e))
+
+    threads = [threading.Thread(target=work, args=job) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    for job, w in zip(jobs, want):
+        assert torch.equal(job[3].owner, w)

@@ -564,7 +564,7 @@ __global__ void __launch_bounds__(kRowThreads<GRAD>, kResident<DT, GRAD>) distil
       }
       if (threadIdx.x == 0) {
         double loss = said.plogp - (dot.x - said.sum * (double)logf(all.s));
-        if (all.s == 0.0f) loss = said.sum > 0.0 ? (double)__int_as_float(0x7f800000) : 0.0;
+        if (all.s == 0.0f) loss = said.sum > 0.0 ? (double)__int_as_float(0x7f800000) : said.sum;  // 0, or the teacher's NaN
         if (tail > 0.0f) loss += (double)(tail * (logf(tail) - (logf(rest.s) + lead - logf(all.s))));
         static_cast<float*>(a.loss.data)[row_at(a.g, a.loss, r)] = (float)loss;
       }

@@ -48,3 +48,22 @@ def test_long_rows_from_threads(ctx):
     assert not failed, failed
     for job, w in zip(jobs, want):
         assert torch.equal(job[3].owner, w)
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("unit", [True, False])
+def test_nan_of_a_teacher_shows(ctx, tail, unit):
+    """A NaN among a teacher's entries makes the loss NaN, also where the student's row is masked throughout."""
+    x = torch.randn(3, 500, device="cuda")
+    x[1] = -float("inf")
+    ids = torch.arange(3, device="cuda").int().expand(3, 3).contiguous()
+    z = torch.full((3, 3), -2.0, device="cuda")
+    z[:2, 1] = float("nan")
+    if not unit:
+        x = x.t().contiguous().t()
+    only, loss, dx = torch.zeros(3, device="cuda"), torch.zeros(3, device="cuda"), torch.zeros_like(x)
+    torch.cuda.synchronize()
+    lb.distill_loss(ctx, x, ids, z, 1.0, only, tail=tail)
+    lb.distill_grad(ctx, x, ids, z, 1.0, dx, loss=loss, tail=tail)
+    for got in (only, loss):
+        assert got.isnan().tolist() == [True, True, False]

@@ -621,19 +621,22 @@ uint32_t cluster_of(const lc_context* ctx, uint64_t rows, uint64_t vecs) {
   return cluster;
 }
 
+// Whether a cluster's shared memory holds the bits of a row of `vocab` places.
+bool bits_fit(uint64_t vocab, int32_t dtype) { return vocab / (dtype == LC_F32 ? 4 : 8) <= (kMaxBits - 16) * kMaxCluster; }
+
+// `rows`: by the kernel for rows whose vocabulary is the unit axis and whose bits fit.
 template <int DT, bool GRAD>
-cudaError_t launch(const lc_context* ctx, const DistillArgs& a, bool unit, cudaStream_t stream) {
-  const uint64_t vecs = a.vocab / Vec<DT>::kElems;
-  if (unit && vecs <= (kMaxBits - 16) * kMaxCluster) return launch_rows<DT, GRAD>(ctx, a, cluster_of(ctx, a.g.rows, vecs), stream);
+cudaError_t launch(const lc_context* ctx, const DistillArgs& a, bool rows, cudaStream_t stream) {
+  if (rows) return launch_rows<DT, GRAD>(ctx, a, cluster_of(ctx, a.g.rows, a.vocab / Vec<DT>::kElems), stream);
   distill_strided<DT, GRAD><<<(unsigned)std::min<uint64_t>(a.g.rows, kMaxGrid), kThreads, 0, stream>>>(a);
   return cudaSuccess;
 }
 
 template <bool GRAD>
-cudaError_t launch(const lc_context* ctx, const DistillArgs& a, int32_t dtype, bool unit, cudaStream_t s) {
-  if (dtype == LC_F32) return launch<LC_F32, GRAD>(ctx, a, unit, s);
-  if (dtype == LC_F16) return launch<LC_F16, GRAD>(ctx, a, unit, s);
-  return launch<LC_BF16, GRAD>(ctx, a, unit, s);
+cudaError_t launch(const lc_context* ctx, const DistillArgs& a, int32_t dtype, bool rows, cudaStream_t s) {
+  if (dtype == LC_F32) return launch<LC_F32, GRAD>(ctx, a, rows, s);
+  if (dtype == LC_F16) return launch<LC_F16, GRAD>(ctx, a, rows, s);
+  return launch<LC_BF16, GRAD>(ctx, a, rows, s);
 }
 
 lc_status distill(const char* op, lc_context* ctx, void* stream, const lc_view* logits, const lc_view* ids,
@@ -677,10 +680,11 @@ lc_status distill(const char* op, lc_context* ctx, void* stream, const lc_view* 
   DeviceGuard on(ctx->device);
   cudaStream_t s = stream_of(ctx, stream);
   const bool unit = a.vocab == 1 || (a.x.inner == 1 && (!dlogits || a.dx.inner == 1));
-  const cudaError_t e = dlogits ? launch<true>(ctx, a, logits->dtype, unit, s) : launch<false>(ctx, a, logits->dtype, unit, s);
+  const bool rows = unit && bits_fit(a.vocab, logits->dtype);
+  const cudaError_t e = dlogits ? launch<true>(ctx, a, logits->dtype, rows, s) : launch<false>(ctx, a, logits->dtype, rows, s);
   if (e != cudaSuccess) return cuda_fail(e, op);
-  return launched(ctx, dlogits ? (unit ? "distill_grad_rows" : "distill_grad_strided")
-                               : (unit ? "distill_loss_rows" : "distill_loss_strided"));
+  return launched(ctx, dlogits ? (rows ? "distill_grad_rows" : "distill_grad_strided")
+                               : (rows ? "distill_loss_rows" : "distill_loss_strided"));
 }
 
 }  // namespace

@@ -67,3 +67,15 @@ def test_nan_of_a_teacher_shows(ctx, tail, unit):
     lb.distill_grad(ctx, x, ids, z, 1.0, dx, loss=loss, tail=tail)
     for got in (only, loss):
         assert got.isnan().tolist() == [True, True, False]
+
+
+def test_the_kernel_that_ran_is_the_one_recorded(ctx):
+    """A vocabulary too long for a cluster's shared memory goes to the kernel for any strides, and the record says so."""
+    x = torch.zeros(1, 4_300_001, device="cuda", dtype=torch.bfloat16)
+    ids, z = torch.zeros(1, 1, device="cuda").int(), torch.full((1, 1), -1.0, device="cuda")
+    loss, dx = torch.empty(1, device="cuda"), torch.empty_like(x)
+    torch.cuda.synchronize()
+    for n, way in ((x.shape[1], "strided"), (4_000_000, "rows")):
+        lb.distill_loss(ctx, x[:, :n], ids, z, 1.0, loss, tail=True)
+        lb.distill_grad(ctx, x[:, :n], ids, z, 1.0, dx[:, :n], tail=True)
+        assert ctx.debug_launches()[-2:] == [f"distill_loss_{way}", f"distill_grad_{way}"]

@@ -339,7 +339,8 @@ def _stream(stream):
     if stream is None or type(stream) is int:
         return stream
     if hasattr(stream, "cuda_stream"):
-        return stream.cuda_stream
+        # torch's default stream has handle 0, which would name the context's own: cudaStreamLegacy (1) is the same stream
+        return stream.cuda_stream or 1
     return stream
 
 

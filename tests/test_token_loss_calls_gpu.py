@@ -79,3 +79,45 @@ def test_the_kernel_that_ran_is_the_one_recorded(ctx):
         lb.distill_loss(ctx, x[:, :n], ids, z, 1.0, loss, tail=True)
         lb.distill_grad(ctx, x[:, :n], ids, z, 1.0, dx[:, :n], tail=True)
         assert ctx.debug_launches()[-2:] == [f"distill_loss_{way}", f"distill_grad_{way}"]
+
+
+def test_the_default_stream_by_its_object(ctx):
+    """A call on torch's default stream, named by its object, comes after what torch has put there and before what follows."""
+    n, v, k = 64, 30011, 8
+    x = torch.randn(n, v, device="cuda")
+    t = torch.zeros(n, dtype=torch.int32, device="cuda")
+    lp, stats, ids = torch.empty(n, device="cuda"), torch.empty(n, 2, device="cuda"), torch.empty(n, k, device="cuda").int()
+    late, dx, work = torch.zeros_like(x), torch.empty_like(x), torch.empty(1 << 28, device="cuda")
+    stream = torch.cuda.current_stream()
+    assert stream.cuda_stream == 0
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(2):
+        late.zero_()
+        for _ in range(4):
+            work.zero_()  # a millisecond or so in which a kernel on another stream would read the zeros
+        late.copy_(x)
+        lb.encode_token_logprobs(ctx, stream, late, t, 1.0, logprob=lp, stats=stats, top_ids=ids)
+        lb.encode_token_logprobs_backward(ctx, stream, late, t, 1.0, stats, lp, dx)
+        got.append([y.clone() for y in (lp, stats, ids, dx)])
+        late.zero_()
+    want = torch.log_softmax(x.double(), 1)
+    assert torch.equal(got[0][2].long(), x.topk(k, 1).indices)
+    assert (got[0][0].double() - want[:, 0]).abs().max() < 1e-4
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_products_on_the_default_stream(ctx):
+    """The other calls take the same object: products with a split sum among them, which need scratch."""
+    stream = torch.cuda.current_stream()
+    for dtype, (m, n, k) in ((torch.float32, (96, 64, 20000)), (torch.bfloat16, (128, 256, 16384)), (torch.bfloat16, (100, 36, 52))):
+        a, b = torch.randn(m, k, device="cuda").to(dtype), torch.randn(k, n, device="cuda").to(dtype)
+        own, c = (torch.zeros(m, n, device="cuda", dtype=dtype) for _ in range(2))
+        turned = torch.zeros(n, m, device="cuda")
+        torch.cuda.synchronize()
+        lb.gemm(ctx, 1.0, a, b, 0.0, own)
+        lb.encode_gemm(ctx, stream, 1.0, a, b, 0.0, c)
+        lb.encode_materialize(ctx, stream, c.float().t(), turned)
+        again = turned.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(c, own) and torch.equal(again, c.float().t())

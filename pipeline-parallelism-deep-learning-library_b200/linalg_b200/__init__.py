@@ -235,7 +235,10 @@ def _view_of(t, dtype: int | None = None) -> lc_view:
         return lc_view.from_buffer_copy(_pack_view(st.data_ptr(), st.nbytes(), t.storage_offset(), code, rank, *shape, *none,
                                                    *strides, *none))
     except struct.error:
-        raise InvalidArgument(ERR_INVALID_ARGUMENT, "negative stride") from None
+        if not hasattr(code, "__index__"):
+            raise TypeError(f"element type {code!r} is not a code of this module") from None
+        raise InvalidArgument(ERR_INVALID_ARGUMENT,
+                              "negative stride" if min(strides, default=0) < 0 else f"unknown element type {code}") from None
 
 
 class View:

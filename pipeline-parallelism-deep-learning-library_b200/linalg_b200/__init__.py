@@ -535,15 +535,14 @@ def relu_backward(ctx, pre, dy, dx, stream=None):
 # ---------------------------------------------------------------------------------------------
 
 def _arg(ctx: Context, x):
-    """An operand as the C calls take it: a view by reference, or NULL for one that is not there.  A tensor has to
-    lie on the context's device; a kernel that followed the address of any other would fault."""
+    """An operand as the C calls take it: a view by reference, or NULL for one that is not there.  A tensor, or the one
+    that a view is of, has to lie on the context's device; a kernel that followed the address of any other would fault."""
     if x is None:
         return None
-    if isinstance(x, View):
-        return x.c
-    if x.get_device() != ctx.device:
-        raise InvalidArgument(ERR_INVALID_ARGUMENT, f"operand on {x.device}, not on the context's device cuda:{ctx.device}")
-    return _view_of(x)
+    t = x.owner if isinstance(x, View) else x
+    if (t is x or hasattr(t, "get_device")) and t.get_device() != ctx.device:
+        raise InvalidArgument(ERR_INVALID_ARGUMENT, f"operand on {t.device}, not on the context's device cuda:{ctx.device}")
+    return _view_of(x) if t is x else x.c
 
 
 def encode_token_logprobs(ctx: Context, stream, logits, targets, scale=1.0, logprob=None, entropy=None, stats=None,

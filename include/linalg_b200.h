@@ -266,8 +266,8 @@ lc_status lc_relu_backward(lc_context* ctx, void* stream, const lc_view* pre, co
 /* ---- scores and losses over a vocabulary (no reference counterpart) --------------------------- */
 /* `logits` is [..., V] of f32, f16 or bf16 with any strides: the last axis is the vocabulary (1 to
  * 2^31 - 1 places), the leading axes are the rows.  The softmax is that of scale * logits, scale
- * positive and finite (the inverse of a temperature); sums and statistics are f32 or wider.  Every
- * other operand has the logits' leading shape, with one axis more where one is named.  Indices are
+ * positive and at most 2^100 (the inverse of a temperature); sums and statistics are f32 or wider.
+ * Every other operand has the logits' leading shape, with one axis more where one is named.  Indices are
  * i32 or u32; one outside [0, V), -1 among them, stands for no token.  Errors are the op API's
  * (LC_ERR_INVALID_ARGUMENT, LC_ERR_OVERLAP); no output may overlap an input or another output, but
  * dlogits may be the logits themselves (same buffer, offset, shape and strides).  The calls

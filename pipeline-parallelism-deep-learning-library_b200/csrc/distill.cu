@@ -12,8 +12,6 @@
 //   scale (c q_j - P_k) at the place of entry k,   scale q_j (c - r / Q) outside the list.
 // Outside the list everything is measured from the largest logit there (mt, with St = sum e^(scale (x - mt))): the second
 // form is e^(scale (x_j - mt)) (c e^(scale (mt - m)) / S - r / St), which stands also where Q underflows.
-#include <cmath>
-
 #include "vocab.cuh"
 
 namespace {
@@ -646,7 +644,7 @@ lc_status distill(const char* op, lc_context* ctx, void* stream, const lc_view* 
   Call c(op, logits);
   lc_status st = c.start();
   if (st) return st;
-  if (!std::isfinite(scale) || !(scale > 0.0f)) return c.bad("scale must be positive and finite");
+  if ((st = c.check_scale(scale))) return st;
   if (tail != 0 && tail != 1) return c.bad("tail is 0 (renormalised) or 1 (a bucket for the rest)");
   if (!ids || !teacher) return c.bad("null ids or teacher");
   if (ids->rank != logits->rank) return c.bad("ids must have the logits' leading shape and an axis of their own");

@@ -3,8 +3,6 @@
 //
 // With d_j = scale (x_j - m), m = max x and L = log sum e^d:  log p_j = d_j - L,  H = L - (sum e^d d) / (sum e^d).
 // Gradient for g = d(total)/d(log p_t) and h = d(total)/dH:  dx_j = scale (g ([j = t] - p_j) - h p_j (log p_j + H)).
-#include <cmath>
-
 #include "vocab.cuh"
 
 namespace {
@@ -655,8 +653,6 @@ lc_status launched(lc_context* ctx, const char* name) {
   return LC_OK;
 }
 
-bool good_scale(float s) { return std::isfinite(s) && s > 0.0f; }
-
 // How a row is spread: blocks of `threads` in a cluster of `cluster`, and the slots of its alternatives.
 struct Spread {
   uint32_t cluster, threads, n_slots, per_slot;
@@ -747,7 +743,7 @@ lc_status lc_encode_token_logprobs(lc_context* ctx, void* stream, const lc_view*
   Call c("token_logprobs", logits);
   lc_status st = c.start();
   if (st) return st;
-  if (!good_scale(scale)) return c.bad("scale must be positive and finite");
+  if ((st = c.check_scale(scale))) return st;
   if (!logprob && !entropy && !stats && !top_logprobs && !top_ids) return c.bad("no output asked for");
   if ((targets == nullptr) != (logprob == nullptr)) return c.bad("targets and logprob come together");
   const lc_view* top = top_ids ? top_ids : top_logprobs;
@@ -801,7 +797,7 @@ lc_status lc_encode_token_logprobs_backward(lc_context* ctx, void* stream, const
   Call c("token_logprobs_backward", logits);
   lc_status st = c.start();
   if (st) return st;
-  if (!good_scale(scale)) return c.bad("scale must be positive and finite");
+  if ((st = c.check_scale(scale))) return st;
   if (!stats || !dlogits) return c.bad("null stats or dlogits");
   if (!d_logprob && !d_entropy) return c.bad("neither d_logprob nor d_entropy given");
   if (d_logprob && !targets) return c.bad("d_logprob needs the targets");

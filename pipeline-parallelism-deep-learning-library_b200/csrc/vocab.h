@@ -5,6 +5,7 @@
 // the rows.  Every other operand has the same leading axes, and at most one axis more.
 #pragma once
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <string>
 
@@ -14,6 +15,7 @@ namespace lcv {
 
 constexpr int kMaxOperands = 8;       // operands of one call beside the logits
 constexpr uint64_t kMaxVocab = 0x7fffffffull;
+constexpr float kMaxScale = 0x1p100f;
 
 // The leading axes, merged where every operand steps uniformly over two of them.
 struct Rows {
@@ -72,6 +74,14 @@ class Call {
     if (x_->rank < 1) return bad("logits need a vocabulary axis");
     if (vocab() == 0) return bad("the vocabulary is empty");
     if (vocab() > kMaxVocab) return bad("the vocabulary exceeds 2^31 - 1");
+    return LC_OK;
+  }
+
+  // Far below where scale * log2(e) (2.3e38) or an entropy's gradient times a far place's d (3e34) would leave f32 and make
+  // NaN of 0 * infinity.
+  lc_status check_scale(float scale) const {
+    if (!std::isfinite(scale) || !(scale > 0.0f)) return bad("scale must be positive and finite");
+    if (scale > kMaxScale) return bad("scale must be at most 2^100");
     return LC_OK;
   }
 

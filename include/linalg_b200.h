@@ -284,7 +284,9 @@ lc_status lc_relu_backward(lc_context* ctx, void* stream, const lc_view* pre, co
  *                            for the gradient
  *   top_logprobs [..., K] f32, top_ids [..., K]   the K largest logits' log probabilities and
  *                            places, best first; equal logits by the lower place, a NaN above every
- *                            number.  1 <= K <= 128, K <= V */
+ *                            number.  1 <= K <= 128, K <= V
+ * A vocabulary that is the unit axis is read once; with any other stride the alternatives read it
+ * once more each. */
 lc_status lc_encode_token_logprobs(lc_context* ctx, void* stream, const lc_view* logits,
                                    const lc_view* targets, float scale, const lc_view* logprob,
                                    const lc_view* entropy, const lc_view* stats,

@@ -209,14 +209,18 @@ __global__ void __launch_bounds__(kThreads) distill_strided(DistillArgs a) {
 // the second one that lets it go, and the gradient is stored past the caches.
 //
 // What bounds it (B200, of the 6465 GB/s of a copy).  The loss alone reads HBM at 6128 GB/s (4096 x 131,072 bf16, 64 entries:
-// 176 us).  With the gradient it is 446 us, 4818 GB/s of the bytes that must move: 1.16 times the logits come from HBM
+// 176 us).  With the gradient it is 450 us, 4780 GB/s of the bytes that must move: 1.15 times the logits come from HBM
 // (some lines are gone before the second pass), and a block's chain from its list over the sums to the gradient leaves the
-// memory idle where the other block of its SM cannot fill in.  A fetch of the row's first half into L2 before the list took
-// 454 to 446 us (4096 x 32,768 f32: 203 to 192); of the whole row, 509; on short rows and for the loss alone it cost time.  Tried and slower: the row in shared memory over a cluster of
-// 8 blocks filled by the copy engine, one pass after the other (755 us) or with the next row's sums before this row's
-// gradient (811 us; the fixed work of a block weighs 8 times); the first 88 KB of a row in shared memory (527 us); lists a
-// row ahead and gradient tiles to whichever warp is free (486 us); three or four smaller blocks an SM (505 to 521 us: more
-// rows under way than L2 holds).
+// memory idle where the other block of its SM cannot fill in.  A fetch of the row's first 128 KB (half of it) into L2 before
+// the list took 454 to 446 us (4096 x 32,768 f32: 203 to 192); of the whole row, 509; on short rows and for the loss alone it
+// cost time.  Tried and slower: the row in shared memory over a cluster of 8 blocks filled by the copy engine, one pass after
+// the other (755 us) or with the next row's sums before this row's gradient (811 us; the fixed work of a block weighs 8
+// times); the first 88 KB of a row in shared memory (527 us); lists a row ahead and gradient tiles to whichever warp is free
+// (486 us); three or four smaller blocks an SM (505 to 521 us: more rows under way than L2 holds).
+// Rows from about 400 KB on are too long for that: 296 of them are more than L2's 126 MB, and most of the second pass comes
+// from HBM too (2048 x 131,072 f32: 474 us, floor 332; over 1024 such rows 1.73 times the logits are read).
+// Many short rows with long lists are bound by the fixed work of a row, its list above all (8000 x 2001 bf16: 38 us with 16
+// entries, 70 with 128, floor 10 and 11; the loss alone with 128: 50).
 template <int DT>
 constexpr int kUnroll = 32 / Vec<DT>::kElems;  // vectors of a step: 32 places a thread
 template <bool GRAD>
@@ -587,7 +591,8 @@ cudaError_t launch_rows(const lc_context* ctx, const DistillArgs& a, uint32_t cl
   const uint64_t share = std::max<uint64_t>(16, ((vecs + cluster - 1) / cluster + 15) / 16 * 16);
   const uint64_t busy = std::max<uint64_t>((share + kUnroll<DT> - 1) / kUnroll<DT>, a.list);
   // long slices: two blocks of 512 threads an SM, so that most of the rows under way stay in L2 for their second pass (4096 x
-  // 131,072 bf16: 463 us, 505 with four of 256); shorter ones: four of 256 (777 x 50,001 bf16: 54.6 us, 59.5 with two of 512)
+  // 131,072 bf16: 463 us, 505 with four of 256), as far as L2 goes: rows above 400 KB or so do not fit either way; shorter
+  // ones: four of 256 (777 x 50,001 bf16: 54.6 us, 59.5 with two of 512)
   const uint64_t most = share * 16 < kLongSlice ? 256 : kRowThreads<GRAD>;
   const uint32_t threads = (uint32_t)std::min<uint64_t>(most, std::max<uint64_t>(32, (busy + 31) / 32 * 32));
   const bool moved = GRAD && apart(a.g, a.x, a.dx, 16 / kE);

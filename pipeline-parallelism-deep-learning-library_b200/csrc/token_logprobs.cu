@@ -46,7 +46,8 @@ __device__ __forceinline__ void write_best(const ScoreArgs& a, uint64_t r, uint3
 }
 
 // One block a row, every element read where its stride puts it: once for the maximum and the sums, and once more for each
-// alternative asked for.
+// alternative asked for, so that many of them are dear: 512 x 50,001 bf16 with the vocabulary as the outer axis 108 us, 2.2 ms
+// with 20 alternatives, 13.3 ms with 128.
 template <int DT>
 __global__ void __launch_bounds__(kThreads) token_logprobs_strided(ScoreArgs a) {
   using E = Elem<DT>;
@@ -101,13 +102,13 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_strided(ScoreArgs a) 
 // the K-th largest order bit by bit instead: right for every row, and slower.
 //
 // What bounds it (B200, whole call in a graph, of the 6465 GB/s of a copy): HBM.  2048 x 100,003 f32 with entropy reads at
-// 6448 GB/s (127 us), 4096 x 131,072 bf16 at 6256 (172 us); f16 and bf16 have two exponentials for each of f32 and three
-// quarters of the exponential unit's rate at that speed.  The alternatives cost 26 us more with K = 20 (198 us; 208 with the
-// entropy too): a block waits for one more read from L2 and some barriers, which the other blocks of its SM cover in part.
+// 6439 GB/s (127 us), 4096 x 131,072 bf16 at 6436 (167 us); f16 and bf16 have two exponentials for each of f32 and three
+// quarters of the exponential unit's rate at that speed.  With K = 20 alternatives the latter takes 208 us (198 without the
+// entropy): a block waits for one more read from L2 and some barriers, which the other blocks of its SM cover in part.
 // Why small blocks and not a ring of stages that the copy engine fills (3 of 32 KB a block, two blocks of 512 an SM,
 // measured: 224 us against 182 with four blocks of 256 and plain loads, 173 with six): a block's end is a chain of barriers,
 // and only other blocks can fill it.
-// A single row (1 x 131,072 bf16, K = 20) takes 9.8 us over a cluster of 8, nearly all of it latency: 1.4 us to the logits,
+// A single row (1 x 131,072 bf16, K = 20) takes 9.7 us over a cluster of 8, nearly all of it latency: 1.4 us to the logits,
 // 0.7 to merge, 3.6 for the block's alternatives, the rest for the cluster's.  16 blocks a cluster measured 13.5 us.
 constexpr int kMaxThreads = 256;
 template <int DT>
@@ -562,15 +563,17 @@ __device__ __forceinline__ uint4 grad_vec(const uint4& q, uint32_t j, const Grad
 }
 
 // The vocabulary as the unit axis: a block has `steps` steps of kGradUnroll vectors a thread of one row, with all of a
-// step's loads on the way before the first is used.  The vectors are those of
-// dx, so that every store is a whole one.  MOVED: some row of x starts elsewhere within 16 bytes (an odd vocabulary against
-// padded rows).  A vector of it then is cut out of two aligned ones, of which the second comes from the next lane (a
-// warp's vectors of a step follow one another), or at the end of a warp's vectors from a load of its own.  In steps that reach the row's ends the vectors are read one by one, as
-// are the places around them.
-// Bound by HBM: 4096 x 131,072 bf16 with the entropy's share 331 us, 6495 GB/s, as fast as a copy; stores that stream past
+// step's loads on the way before the first is used.  The vectors are those of dx, so that every store is a whole one.
+// MOVED: some row of x starts elsewhere within 16 bytes (an odd vocabulary against padded rows).  A vector of it then is cut
+// out of two aligned ones, of which the second comes from the next lane (a warp's vectors of a step follow one another), or at
+// the end of a warp's vectors from a load of its own.  In steps that reach the row's ends the vectors are read place by place,
+// as are the places around them.
+// Bound by HBM: 4096 x 131,072 bf16 with the entropy's share 330 us, 6515 GB/s, as fast as a copy; stores that stream past
 // the caches and four blocks an SM with registers enough for all loads of a step (434 us with six and spills).  MOVED rows
-// (1001 x 50,001 bf16 in padded rows: 43 us, 4650 GB/s; 37 us were the rows alike) pay for the shifts, which keep the ALU
-// busy; two loads a vector instead of the neighbour's half measured 53 us.
+// (1001 x 50,001 bf16 in padded rows: 43 us, 4650 GB/s; 37 us were the rows alike) pay for the shifts and, more the shorter
+// the row, for its first and last step, all of whose vectors are read place by place although only the outermost ones reach
+// out of the row (1001 x 131,073: 95 us, 85 alike).  No pipe is full (ALU 42%, issue 50%).  Two loads a vector instead of the
+// neighbour's half measured 53 us.
 constexpr int kGradUnroll = 4;
 
 template <int DT, bool ENT, bool MOVED>

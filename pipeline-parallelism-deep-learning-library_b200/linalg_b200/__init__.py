@@ -343,7 +343,7 @@ def _stream(stream):
         return stream
     if hasattr(stream, "cuda_stream"):
         # torch's default stream has handle 0, which would name the context's own: cudaStreamLegacy (1) is the same stream
-        return stream.cuda_stream or 1
+        return 1 if stream.cuda_stream == 0 else stream.cuda_stream
     return stream
 
 

@@ -18,3 +18,7 @@ def test_a_stream_object_names_its_own_stream():
 def test_none_and_handles_are_as_they_were():
     assert lb._stream(None) is None
     assert lb._stream(0) == 0 and lb._stream(1) == 1 and lb._stream(0x7f00) == 0x7f00
+
+
+def test_an_object_without_a_handle_names_the_contexts_stream():
+    assert lb._stream(Stream(None)) is None
